@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libbitllm_hip.so")
 W_TERNARY, W_INT8, W_INT4 = 1, 2, 3
 PATH_AUTO, PATH_GEMV, PATH_GEMM = 0, 1, 2
 
-_vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_vp, _i, _f, _sz, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64
 
 PRE_NONE, PRE_RMS, PRE_SWIGLU_RMS = 0, 1, 2
 
@@ -63,6 +63,14 @@ _SIGS = {
     "eif_hip_qlinear_prep_acc": (_i, [_vp, C.POINTER(PrepSpec), _vp, _i, _vp]),
     "eif_hip_prep_spec_rows": (_i, [C.POINTER(PrepSpec), _i, _vp, _i, _vp, _i, _vp]),
     "eif_hip_quant_rows": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "eif_hip_mx4_kpad": (_i, [_i]),
+    "eif_hip_mx4_quant_rows": (_i, [_vp, _i, _i64, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "eif_hip_mx4_weight_create": (_i, [C.POINTER(_vp), _i, _i, _i, _vp, _i64, _vp, _i64, _i, _vp]),
+    "eif_hip_mx4_weight_destroy": (None, [_vp]),
+    "eif_hip_mx4_weight_info": (_i, [_vp, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i), C.POINTER(_i), C.POINTER(_sz)]),
+    "eif_hip_mx4_linear": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i, _vp, _i64, _i, _vp]),
+    "eif_hip_mx4_linear_rows": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i64, _i, _vp]),
+    "eif_hip_mx4_linear_grouped": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
     "eif_gguf_ternary_rows": (_i, [_i, _vp, _i, _i, _vp, _vp]),
     "eif_hip_qweight_from_gguf_ternary": (_i, [_vp, _i, _vp, _i, _i, _vp]),
     "eif_hip_bitnet_create": (_i, [C.POINTER(_vp), C.POINTER(BitnetConfig)]),
@@ -291,6 +299,85 @@ def quant_rows(x, bits, dst, scales, stream=None):
     rows, cols = x.shape
     check(load().eif_hip_quant_rows(ptr(x), x.stride(0), rows, cols, bits, ptr(dst), ptr(scales), stream_ptr(stream)),
           "eif_hip_quant_rows")
+
+
+F32, F16, BF16 = 0, 1, 2   # element types of rows (include/eif_hip_mx.h)
+
+
+def _row_type(t):
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
+
+
+def mx4_kpad(cols):
+    return load().eif_hip_mx4_kpad(cols)
+
+
+def mx4_quant_rows(x, codes=None, scales=None, values=None, stream=None):
+    """Rows x [rows, cols] (device) -> MXFP4 codes [rows, >= kpad / 2] and scales [rows, >= kpad / 32] (uint8), and/or
+    the float32 values they stand for."""
+    rows, cols = x.shape
+    ld = lambda t: 0 if t is None else t.stride(0)   # noqa: E731
+    check(load().eif_hip_mx4_quant_rows(ptr(x), _row_type(x), ld(x), rows, cols, ptr(codes), ld(codes), ptr(scales),
+                                        ld(scales), ptr(values), ld(values), stream_ptr(stream)),
+          "eif_hip_mx4_quant_rows")
+
+
+class Mx4Weight:
+    """MXFP4 matrices [rows, cols] resident in HBM in the GPU layout (include/eif_hip_mx.h), one or a stack of `experts`.
+    codes [(experts,) rows, >= (cols + 1) / 2] and scales [(experts,) rows, >= (cols + 31) / 32]: torch tensors on the
+    device or numpy arrays, uint8, their rows evenly spaced."""
+
+    def __init__(self, rows, cols, codes, scales, experts=1, stream=None):
+        lib, on_device = load(), hasattr(codes, "data_ptr")
+        if on_device != hasattr(scales, "data_ptr"):
+            raise HipError("Mx4Weight: codes and scales are both on the device or both on the host")
+
+        def row_stride(t):
+            s = [t.stride(i) if on_device else t.strides[i] for i in range(len(t.shape))]
+            if t.shape != ((experts, rows, t.shape[-1]) if len(s) == 3 else (experts * rows, t.shape[-1])) or s[-1] != 1:
+                raise HipError(f"Mx4Weight: {tuple(t.shape)} is not {experts} x {rows} rows of bytes")
+            if len(s) == 3 and experts > 1 and s[0] != rows * s[1]:
+                raise HipError("Mx4Weight: the matrices' rows are not evenly spaced")
+            return s[-2]
+
+        h = C.c_void_p()
+        check(lib.eif_hip_mx4_weight_create(C.byref(h), experts, rows, cols, ptr(codes), row_stride(codes), ptr(scales),
+                                            row_stride(scales), 1 if on_device else 0,
+                                            stream_ptr(stream) if on_device else None), "eif_hip_mx4_weight_create")
+        self.h, self.rows, self.cols, self.experts = h, rows, cols, experts
+        k, b = C.c_int(), C.c_size_t()
+        check(lib.eif_hip_mx4_weight_info(h, None, None, None, C.byref(k), C.byref(b)), "eif_hip_mx4_weight_info")
+        self.kpad, self.bytes = k.value, b.value
+
+    def close(self):
+        if self.h:
+            load().eif_hip_mx4_weight_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def linear(self, codes, scales, y, bias=None, glu=False, stream=None):
+        """y [M, rows or rows / 2] = the product of M quantised rows (mx4_quant_rows)."""
+        check(load().eif_hip_mx4_linear(self.h, ptr(codes), codes.stride(0), ptr(scales), scales.stride(0), ptr(bias),
+                                        int(glu), ptr(y), y.stride(0), y.shape[0], stream_ptr(stream)),
+              "eif_hip_mx4_linear")
+
+    def linear_rows(self, x, y, bias=None, glu=False, stream=None):
+        """The same for M <= 8 unquantised rows x, quantised within the launch."""
+        check(load().eif_hip_mx4_linear_rows(self.h, ptr(x), _row_type(x), x.stride(0), ptr(bias), int(glu), ptr(y),
+                                             y.stride(0), x.shape[0], stream_ptr(stream)), "eif_hip_mx4_linear_rows")
+
+    def linear_grouped(self, codes, scales, offsets, y, row_index=None, bias=None, glu=False, stream=None):
+        """Rows [offsets[e], offsets[e + 1]) of y take matrix e; row i takes the quantised row row_index[i] (None: i)."""
+        check(load().eif_hip_mx4_linear_grouped(self.h, ptr(codes), codes.stride(0), ptr(scales), scales.stride(0),
+                                                codes.shape[0], ptr(row_index), ptr(offsets), ptr(bias), int(glu), ptr(y),
+                                                y.stride(0), y.shape[0], stream_ptr(stream)),
+              "eif_hip_mx4_linear_grouped")
 
 
 class BitnetModel:
