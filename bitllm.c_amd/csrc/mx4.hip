@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "../../include/eif_hip_mx.h"
 
@@ -70,6 +71,41 @@ EIF_DEV float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>
 struct alignas(4 * sizeof(T)) Quad { T v[4]; };
 
+// Columns c .. c + 3 of a row, as they come (loads alone, so that several can be under way) ...
+// VEC: x is aligned to four elements and cols a multiple of four. Columns behind the last are read within the row.
+template <typename T, bool VEC>
+EIF_DEV Quad<T> load4(const T *xr, int c, int cols)
+{
+    if constexpr (VEC) {
+        return *reinterpret_cast<const Quad<T> *>(xr + (c < cols ? c : 0));
+    } else {
+        Quad<T> q;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.v[i] = xr[min(c + i, cols - 1)];
+        return q;
+    }
+}
+// ... and as FP32, zeros behind the last.
+template <typename T>
+EIF_DEV void values4(const Quad<T> &q, int c, int cols, float *v)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? to_f32(q.v[i]) : 0.0f;
+}
+
+// Four values of each lane, a block being eight lanes: the block's scale byte, and the lane's codes.
+EIF_DEV uint32_t quantise4(const float *v, uint32_t &byte)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = umax(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    m = umax(m, __float_as_uint(xlane<1>(__uint_as_float(m))));
+    m = umax(m, __float_as_uint(xlane<2>(__uint_as_float(m))));
+    m = umax(m, __float_as_uint(xlane<4>(__uint_as_float(m))));
+    byte = scale_byte(m);
+    return codes4(v, scale_inverse(byte), byte != 255);
+}
+
 // One wave a row and span: lane l has columns 4 l .. 4 l + 3, a block is eight lanes.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx, int rows, int cols, int spans,
@@ -82,24 +118,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx
     const int span = (int)(unit % spans), c = span * kSpan + lane * 4;
     if (row >= rows) return;
     const T *xr = x + row * ldx;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (VEC && c + 4 <= cols) {
-        const Quad<T> q = *reinterpret_cast<const Quad<T> *>(xr + c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_f32(q.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < cols) v[i] = to_f32(xr[c + i]);
-    }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = umax(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    m = umax(m, __float_as_uint(xlane<1>(__uint_as_float(m))));
-    m = umax(m, __float_as_uint(xlane<2>(__uint_as_float(m))));
-    m = umax(m, __float_as_uint(xlane<4>(__uint_as_float(m))));
-    const uint32_t b = scale_byte(m);
-    const uint32_t q = codes4(v, scale_inverse(b), b != 255);
+    float v[4];
+    values4(load4<T, VEC>(xr, c, cols), c, cols, v);
+    uint32_t b;
+    const uint32_t q = quantise4(v, b);
     if (codes) {
         *reinterpret_cast<uint16_t *>(codes + row * ldc + (c >> 1)) = (uint16_t)q;
         if ((lane & 7) == 0) scales[row * lds + (c >> 5)] = (uint8_t)b;
@@ -176,6 +198,8 @@ struct Mx4Args {
     float *y;
     int64_t ldy;
     int M;
+    int groups;                     // of token rows
+    bool vec;                       // y takes 16-byte stores
     // by expert
     int experts, rows_in;
     const int32_t *index, *offsets;
@@ -183,6 +207,7 @@ struct Mx4Args {
     const void *x;
     int64_t ldx;
     int cols;
+    bool vecx;                      // x takes loads of four elements
 };
 
 // Two MFMAs of one span: codes c0, c1 of a row tile, their scales in bytes 2 h, 2 h + 1 of sw; operand rows' in bytes
@@ -196,7 +221,13 @@ EIF_DEV v4f span_mfma(v4f acc, v4i w0, v4i w1, uint32_t sw, v4i x0, v4i x1, uint
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a1, b1, acc, 4, 4, 2 * H + 1, (int)sw, 1, (int)sx);
 }
 
-EIF_DEV float swiglu(float g, float u) { return (g * (1.0f / (1.0f + expf(-g)))) * u; }
+// SiLU(g) u. v_exp_f32 and v_rcp_f32 are within one unit in the last place; the rounding of -g log2(e) moves the exponential by
+// up to 2^-24 |g| log2(e) of itself, as a rounding of g does, which the sum g has had already.
+EIF_DEV float swiglu(float g, float u)
+{
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * g);
+    return (g * __builtin_amdgcn_rcpf(1.0f + e)) * u;
+}
 
 // The g-th group of TM token rows over the experts' ranges: its expert and its rows [lo, hi); false beyond the last.
 // One wave's lanes take 64 experts at a time; a range is cut to [0, M], so every row is in bounds whatever the offsets.
@@ -224,9 +255,9 @@ EIF_DEV bool find_group(const Mx4Args &a, int g, int &expert, int &lo, int &hi)
             const int l = __ffsll(past) - 1;
             const int at = g - (base + __shfl(sum - groups, l, 64));
             const int s0 = __shfl(s, l, 64), n0 = __shfl(n, l, 64);
-            expert = e0 + l;
-            lo = s0 + at * TM;
-            hi = min(lo + TM, s0 + n0);
+            expert = __builtin_amdgcn_readfirstlane(e0 + l);
+            lo = __builtin_amdgcn_readfirstlane(s0 + at * TM);
+            hi = __builtin_amdgcn_readfirstlane(min(s0 + at * TM + TM, s0 + n0));
             return true;
         }
         base += __shfl(sum, 63, 64);
@@ -234,171 +265,416 @@ EIF_DEV bool find_group(const Mx4Args &a, int g, int &expert, int &lo, int &hi)
     return false;
 }
 
-// One workgroup a row tile (gated: the gate's and the up projection's) and 16 TT token rows; its four waves take the pairs
-// of spans in turn and add their sums up in LDS.
-template <int TT, bool GLU, bool GROUPED>
-__global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4Args a)
+// The biases of a lane's four output rows r0 .. r0 + 3 (gated: gate's, then up's); rows behind the last get some bias.
+template <bool GLU>
+EIF_DEV void load_bias(const float *bias, int r0, int out_rows, float *b0, float *b1)
 {
-    constexpr int NT = GLU ? 2 : 1, TM = 16 * TT;
-    __shared__ v4f red[4][NT * TT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = lane & 15, slot = lane >> 4;
-    const int otiles = GLU ? a.tiles / 2 : a.tiles;
-    const int tile = blockIdx.x % otiles, group = blockIdx.x / otiles;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int r = min(r0 + j, out_rows - 1);
+        b0[j] = bias[r];
+        if (GLU) b1[j] = bias[out_rows + r];
+    }
+}
+
+// The lane's four outputs of a token row. WHOLE: all four exist and y takes a 16-byte store.
+template <bool GLU, bool WHOLE>
+EIF_DEV void store_outputs(float *yr, int r0, int out_rows, v4f s0, v4f s1, const float *b0, const float *b1)
+{
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = s0[j] + b0[j];
+        if (GLU) v[j] = swiglu(v[j], s1[j] + b1[j]);
+    }
+    if (WHOLE) {
+        *reinterpret_cast<float4 *>(yr + r0) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (r0 + j < out_rows) yr[r0 + j] = v[j];
+    }
+}
+
+// Few token rows: what counts is how soon and how much of the matrix is on its way. A workgroup of eight waves takes
+// 8 / KW row tiles (gated: tiles of the gate's and the same of the up projection's) and 16 TT token rows. KW waves share a
+// tile: wave k takes the spans k, k + KW, ..., D at a time with all their loads out at once, and the sums meet in LDS.
+//   X void: quantised operand rows, straight from memory. Else the rows form: every workgroup quantises the (at most 8)
+// rows of X into LDS while its first codes are on their way.
+template <typename X, int TT, int KW, int D, bool GLU, bool GROUPED>
+__global__ __launch_bounds__(512) void mx4_split_kernel(Mx4Args a)
+{
+    constexpr bool ROWS = !std::is_void<X>::value;
+    constexpr int NT = GLU ? 2 : 1, TM = 16 * TT, TW = 8 / KW;
+    __shared__ v4f red[KW == 1 ? 1 : 8][NT * TT][64];
+    extern __shared__ __align__(16) uint8_t staged[];   // rows form: codes [M][spans 128 + 16], then scales [M][spans 8]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, slot = lane >> 4, kw = wave % KW;
+    const int otiles = GLU ? a.tiles / 2 : a.tiles, tblocks = (otiles + TW - 1) / TW;
+    const int group = blockIdx.x / tblocks, tile = (blockIdx.x % tblocks) * TW + wave / KW;
     int expert = 0, lo = group * TM, hi = min(lo + TM, a.M);
     if (GROUPED && !find_group<TM>(a, group, expert, lo, hi)) return;
 
-    const uint8_t *xr[TT];
-    const uint8_t *sr[TT];
-    bool ok[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        const int m = lo + 16 * t + n;
-        int r = m;
-        ok[t] = m < hi;
-        if (GROUPED) {
-            if (ok[t] && a.index) r = a.index[m];
-            ok[t] = ok[t] && r >= 0 && r < a.rows_in;
-        }
-        r = ok[t] ? r : 0;   // row 0 is there to be read; its sums are not stored
-        xr[t] = a.codes + r * a.ldc + slot * 32;
-        sr[t] = a.scales + r * a.lds + slot * 2;
-    }
-    v4f acc[NT][TT] = {};
-    const size_t first = (size_t)expert * a.tiles + tile;
     const uint8_t *wc[NT];
     const uint32_t *ws[NT];
 #pragma unroll
     for (int h = 0; h < NT; ++h) {
-        wc[h] = a.wc + (first + h * otiles) * tile_codes(a.spans) + lane * 16;
-        ws[h] = a.ws + (first + h * otiles) * tile_scales(a.spans) + lane;
+        const size_t t = (size_t)expert * a.tiles + h * otiles + min(tile, otiles - 1);
+        wc[h] = a.wc + t * tile_codes(a.spans);
+        ws[h] = a.ws + t * tile_scales(a.spans);
     }
-    for (int q = wave; 2 * q < a.spans; q += 4) {
-        uint32_t sw[NT];
+    struct Weights {
+        v4i c[NT][2];
+        uint32_t s[NT];
+    };
+    auto load_weights = [&](Weights &f, int p) {
 #pragma unroll
-        for (int h = 0; h < NT; ++h) sw[h] = ws[h][(size_t)q * 64];
+        for (int h = 0; h < NT; ++h) {
+            f.c[h][0] = *reinterpret_cast<const v4i *>(wc[h] + (size_t)p * 2048 + lane * 16);
+            f.c[h][1] = *reinterpret_cast<const v4i *>(wc[h] + (size_t)p * 2048 + 1024 + lane * 16);
+            f.s[h] = ws[h][(size_t)(p >> 1) * 64 + lane];
+        }
+    };
+    // the j-th span of a wave's batch; behind the last one the batch's first again
+    auto batch_span = [&](int p0, int j) { return p0 + j * KW < a.spans ? p0 + j * KW : min(p0, a.spans - 1); };
+    Weights w[D];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int p = 2 * q + s;
-            if (p >= a.spans) break;
-            v4i w[NT][2];
+    for (int j = 0; j < D; ++j) load_weights(w[j], batch_span(kw, j));
+    __builtin_amdgcn_sched_barrier(0);   // the loads go out here
+
+    const uint8_t *xr[TT];
+    const uint8_t *sr[TT];
+    bool ok[TT];
+    if constexpr (ROWS) {
+        const int ldq = a.spans * 128 + 16;   // 16 bytes on from row to row in the banks
+        uint8_t *sc = staged + a.M * ldq;
+        const X *x = static_cast<const X *>(a.x);
+        auto stage = [&](auto vec) {
+            constexpr int U = 4;   // rows and spans that a wave has under way
+            for (int u0 = wave; u0 < a.M * a.spans; u0 += 8 * U) {
+                Quad<X> q[U];
 #pragma unroll
-            for (int h = 0; h < NT; ++h) {
-                w[h][0] = *reinterpret_cast<const v4i *>(wc[h] + (size_t)p * 2048);
-                w[h][1] = *reinterpret_cast<const v4i *>(wc[h] + (size_t)p * 2048 + 1024);
+                for (int i = 0; i < U; ++i) {
+                    const int u = min(u0 + 8 * i, a.M * a.spans - 1);
+                    q[i] = load4<X, decltype(vec)::value>(x + u / a.spans * a.ldx, u % a.spans * kSpan + lane * 4, a.cols);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int u = u0 + 8 * i, row = u / a.spans, c = u % a.spans * kSpan + lane * 4;
+                    if (u >= a.M * a.spans) break;
+                    float v[4];
+                    values4(q[i], c, a.cols, v);
+                    uint32_t b;
+                    const uint32_t code = quantise4(v, b);
+                    *reinterpret_cast<uint16_t *>(staged + row * ldq + (c >> 1)) = (uint16_t)code;
+                    if ((lane & 7) == 0) sc[row * a.spans * 8 + (c >> 5)] = (uint8_t)b;
+                }
             }
+        };
+        if (a.vecx)
+            stage(std::true_type{});
+        else
+            stage(std::false_type{});
+        __syncthreads();
+        ok[0] = n < a.M;
+        const int row = ok[0] ? n : 0;
+        xr[0] = staged + row * ldq + slot * 32;
+        sr[0] = sc + row * a.spans * 8 + slot * 2;
+    } else {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int m = lo + 16 * t + n;
+            int r = m;
+            ok[t] = m < hi;
+            if (GROUPED) {
+                if (ok[t] && a.index) r = a.index[m];
+                ok[t] = ok[t] && r >= 0 && r < a.rows_in;
+            }
+            r = ok[t] ? r : 0;   // row 0 is there to be read; its sums are not stored
+            xr[t] = a.codes + r * a.ldc + slot * 32;
+            sr[t] = a.scales + r * a.lds + slot * 2;
+        }
+    }
+    v4f acc[NT][TT] = {};
+    for (int p0 = kw; p0 < a.spans; p0 += KW * D) {
+        v4i x[D][TT][2];
+        uint32_t sx[D][TT];
+        if (p0 != kw) {
+#pragma unroll
+            for (int j = 0; j < D; ++j) load_weights(w[j], batch_span(p0, j));
+        }
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+            const int p = batch_span(p0, j);
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                const v4i x0 = *reinterpret_cast<const v4i *>(xr[t] + (size_t)p * 128);
-                const v4i x1 = *reinterpret_cast<const v4i *>(xr[t] + (size_t)p * 128 + 16);
-                const uint32_t sx = *reinterpret_cast<const uint16_t *>(sr[t] + p * 8);
-#pragma unroll
-                for (int h = 0; h < NT; ++h)
-                    acc[h][t] = s == 0 ? span_mfma<0>(acc[h][t], w[h][0], w[h][1], sw[h], x0, x1, sx)
-                                       : span_mfma<1>(acc[h][t], w[h][0], w[h][1], sw[h], x0, x1, sx);
+                x[j][t][0] = *reinterpret_cast<const v4i *>(xr[t] + (size_t)p * 128);
+                x[j][t][1] = *reinterpret_cast<const v4i *>(xr[t] + (size_t)p * 128 + 16);
+                sx[j][t] = *reinterpret_cast<const uint16_t *>(sr[t] + (size_t)p * 8);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+            const int p = p0 + j * KW;
+            if (p >= a.spans) break;
+#pragma unroll
+            for (int h = 0; h < NT; ++h)
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                    acc[h][t] = span_mfma<0>(acc[h][t], w[j].c[h][0], w[j].c[h][1], w[j].s[h] >> (16 * (p & 1)), x[j][t][0],
+                                             x[j][t][1], sx[j][t]);
+        }
     }
-#pragma unroll
-    for (int h = 0; h < NT; ++h)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) red[wave][h * TT + t][lane] = acc[h][t];
-    __syncthreads();
-    const int out_rows = GLU ? a.rows / 2 : a.rows;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        if (t % 4 != wave || !ok[t]) continue;
-        v4f s[NT];
+    if (KW > 1) {
 #pragma unroll
         for (int h = 0; h < NT; ++h)
-            s[h] = ((red[0][h * TT + t][lane] + red[1][h * TT + t][lane]) + red[2][h * TT + t][lane]) + red[3][h * TT + t][lane];
-        float *yr = a.y + (int64_t)(lo + 16 * t + n) * a.ldy;
-        const float *bias = a.bias ? a.bias + (size_t)expert * a.rows : nullptr;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = tile * 16 + slot * 4 + i;
-            if (r >= out_rows) continue;
-            float v = s[0][i] + (bias ? bias[r] : 0.0f);
-            if (GLU) v = swiglu(v, s[NT - 1][i] + (bias ? bias[out_rows + r] : 0.0f));
-            yr[r] = v;
+            for (int t = 0; t < TT; ++t) red[KW == 1 ? 0 : wave][h * TT + t][lane] = acc[h][t];
+        __syncthreads();
+    }
+    if (tile >= otiles) return;
+    const int out_rows = GLU ? a.rows / 2 : a.rows, r0 = tile * 16 + slot * 4;
+    float b0[4] = {}, b1[4] = {};
+    if (a.bias) load_bias<GLU>(a.bias + (size_t)expert * a.rows, r0, out_rows, b0, b1);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        if (KW > 1) {   // the waves of a tile take its token tiles in turn
+            if (t % KW != kw) continue;
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                acc[h][t] = red[wave - kw][h * TT + t][lane];
+#pragma unroll
+                for (int k = 1; k < KW; ++k) acc[h][t] += red[wave - kw + k][h * TT + t][lane];
+            }
         }
+        if (!ok[t]) continue;
+        float *yr = a.y + (int64_t)(lo + 16 * t + n) * a.ldy;
+        if (a.vec && r0 + 4 <= out_rows)
+            store_outputs<GLU, true>(yr, r0, out_rows, acc[0][t], acc[NT - 1][t], b0, b1);
+        else
+            store_outputs<GLU, false>(yr, r0, out_rows, acc[0][t], acc[NT - 1][t], b0, b1);
     }
 }
 
-// The rows form: every workgroup quantises the token rows into LDS, then takes a row tile as above.
-template <typename T, bool GLU>
-__global__ __launch_bounds__(256) void mx4_rows_kernel(Mx4Args a)
+// 16 bytes from memory straight into LDS, lane l's behind lane l - 1's.
+EIF_DEV void load_lds16(const void *src, void *dst)
 {
-    constexpr int NT = GLU ? 2 : 1;
-    __shared__ v4f red[4][NT][64];
-    extern __shared__ __align__(16) uint8_t staged[];   // codes [M][ldq], then scales [M][kpad / 32]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
+// Many token rows: a workgroup of four waves takes 16 TT token rows and 4 RT row tiles, RT to a wave (gated: RT / 2 of the
+// gate's and the same of the up projection's). A wave's row tiles are its own, so their codes go from memory straight
+// into registers; the token rows are shared, so they go into LDS; both PF spans ahead.
+//   A span of a token tile is 16 rows of 128 bytes, 8 pieces h of 16 (piece h = 2 slot + step). A load covers eight rows,
+// whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ (n / 2)) of its half of the tile, so that the 16
+// lanes of a slot, which read one piece of 16 rows, meet 16 different groups of banks.
+template <int RT, int TT, int PF, bool GLU, bool GROUPED>
+__global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx4Args a)
+{
+    constexpr int NT = GLU ? 2 : 1, OT = RT / NT, TM = 16 * TT;
+    constexpr int R = PF + 1, SV = R / 2;       // spans in LDS and registers, pairs of spans of scales under way
+    constexpr int PT = (2 * TT + 3) / 4;        // half tiles of token rows that a wave stages
+    constexpr int PS = (2 * TM + 255) / 256;    // scales that a thread stages: a row's of one span of a pair
+    static_assert(PF == 1 || PF == 3, "the loop below goes by four spans");
+    // spans in turn; an array each: the compiler then knows that a load into one does not touch a read of the other
+    __shared__ v4i xt0[TT * 128], xt1[TT * 128];
+    __shared__ __align__(8) uint16_t xs0[TM * 8], xs1[TM * 8];   // pairs of spans in turn: [row][span of the pair][slot]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, slot = lane >> 4;
-    const int otiles = GLU ? a.tiles / 2 : a.tiles, tile = blockIdx.x;
-    const int ldq = a.spans * 128 + 16;   // 16 bytes on from row to row in the banks
-    uint8_t *sc = staged + a.M * ldq;
-    for (int u = wave; u < a.M * a.spans; u += 4) {
-        const int row = u / a.spans, c = (u % a.spans) * kSpan + lane * 4;
-        const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int otiles = GLU ? a.tiles / 2 : a.tiles;
+    const int rblocks = (otiles + 4 * OT - 1) / (4 * OT);
+    // Workgroups go to the XCDs in turn: each XCD gets a stretch of consecutive ids, ordered in strips of 8 row blocks, so
+    // that what it works on at a time is about as many row blocks as groups of token rows, which meet in its L2.
+    const unsigned per = (gridDim.x + 7) / 8;
+    const unsigned id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (id >= (unsigned)rblocks * a.groups) return;
+    const int strip = id / (8u * a.groups), rest = id % (8u * a.groups), high = min(8, rblocks - 8 * strip);
+    const int rb = 8 * strip + rest % high, group = rest / high;
+    int expert = 0, lo = group * TM, hi = min(lo + TM, a.M);
+    if (GROUPED && !find_group<TM>(a, group, expert, lo, hi)) return;
+    const int last = a.spans - 1;
+
+    struct Weights {
+        v4i c[RT][2];
+        uint32_t s[RT];
+    };
+    Weights w[R];
+    // Row tiles behind the matrix's last (of the last row block) are read too, the allocation holds enough of them, and not
+    // stored. The same for all lanes:
+    const uint32_t tile_c = a.spans * 2048u, tile_s = (a.spans + 1) / 2 * 64u;
+    const uint8_t *wc[NT];
+    const uint32_t *ws[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < a.cols) v[i] = to_f32(xr[c + i]);
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = umax(m, __float_as_uint(v[i]) & 0x7fffffffu);
-        m = umax(m, __float_as_uint(xlane<1>(__uint_as_float(m))));
-        m = umax(m, __float_as_uint(xlane<2>(__uint_as_float(m))));
-        m = umax(m, __float_as_uint(xlane<4>(__uint_as_float(m))));
-        const uint32_t b = scale_byte(m);
-        const uint32_t q = codes4(v, scale_inverse(b), b != 255);
-        *reinterpret_cast<uint16_t *>(staged + row * ldq + (c >> 1)) = (uint16_t)q;
-        if ((lane & 7) == 0) sc[row * a.spans * 8 + (c >> 5)] = (uint8_t)b;
+    for (int h = 0; h < NT; ++h) {
+        const size_t t = (size_t)expert * a.tiles + h * otiles + (rb * 4 + wave) * OT;
+        wc[h] = a.wc + t * tile_c;
+        ws[h] = a.ws + t * tile_s;
     }
-    __syncthreads();
-    const int row = n < a.M ? n : 0;
-    const uint8_t *xr = staged + row * ldq + slot * 32;
-    const uint8_t *sr = sc + row * a.spans * 8 + slot * 2;
-    v4f acc[NT] = {};
-    for (int q = wave; 2 * q < a.spans; q += 4) {
+    auto load_weights = [&](int p, Weights &f) {
 #pragma unroll
-        for (int h = 0; h < NT; ++h) {
-            const size_t t = tile + h * otiles;
-            const uint32_t sw = a.ws[t * tile_scales(a.spans) + (size_t)q * 64 + lane];
+        for (int i = 0; i < RT; ++i) {
+            const uint8_t *src = wc[i / OT] + (i % OT * tile_c + p * 2048u);
+            f.c[i][0] = *reinterpret_cast<const v4i *>(src + lane * 16);
+            f.c[i][1] = *reinterpret_cast<const v4i *>(src + 1024 + lane * 16);
+        }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int p = 2 * q + s;
-                if (p >= a.spans) break;
-                const uint8_t *wp = a.wc + t * tile_codes(a.spans) + (size_t)p * 2048 + lane * 16;
-                const v4i w0 = *reinterpret_cast<const v4i *>(wp), w1 = *reinterpret_cast<const v4i *>(wp + 1024);
-                const v4i x0 = *reinterpret_cast<const v4i *>(xr + p * 128);
-                const v4i x1 = *reinterpret_cast<const v4i *>(xr + p * 128 + 16);
-                const uint32_t sx = *reinterpret_cast<const uint16_t *>(sr + p * 8);
-                acc[h] = s == 0 ? span_mfma<0>(acc[h], w0, w1, sw, x0, x1, sx) : span_mfma<1>(acc[h], w0, w1, sw, x0, x1, sx);
-            }
+        for (int i = 0; i < RT; ++i) f.s[i] = (ws[i / OT] + (i % OT * tile_s + p / 2 * 64u))[lane];
+    };
+#pragma unroll
+    for (int k = 0; k < PF; ++k) load_weights(min(k, last), w[k]);
+
+    auto operand_row = [&](int m) {
+        if (m >= hi) return 0;   // row 0 is there to be read; its sums are not stored
+        if (!GROUPED) return m;
+        const int r = a.index ? a.index[m] : m;
+        return r >= 0 && r < a.rows_in ? r : 0;
+    };
+    // where there are fewer half tiles than waves, or rows than threads, some stage the same
+    const int half0 = PT * wave % (2 * TT);
+    const uint8_t *xr[PT];
+#pragma unroll
+    for (int j = 0; j < PT; ++j) {
+        const int half = half0 + j, r = 8 * (half & 1) + (lane >> 3);
+        xr[j] = a.codes + operand_row(lo + 16 * (half >> 1) + r) * a.ldc + ((lane & 7) ^ (r >> 1)) * 16;
+    }
+    const uint8_t *sr[PS];
+#pragma unroll
+    for (int j = 0; j < PS; ++j) sr[j] = a.scales + operand_row(lo + (j * 256 + (int)threadIdx.x) % (2 * TM) / 2) * a.lds;
+    const int odd_thread = threadIdx.x & 1;
+    // one span ahead: from memory straight into LDS; more: through registers, whose loads the compiler waits for one by one
+    v4i xv[R][PT];
+    auto load_rows = [&](int p, v4i *v, v4i *dst) {
+#pragma unroll
+        for (int j = 0; j < PT; ++j) {
+            if constexpr (PF == 1)
+                load_lds16(xr[j] + (size_t)p * 128, dst + (half0 + j) * 64);
+            else
+                v[j] = *reinterpret_cast<const v4i *>(xr[j] + (size_t)p * 128);
+        }
+    };
+    auto store_rows = [&](const v4i *v, v4i *dst) {
+        if constexpr (PF > 1) {
+#pragma unroll
+            for (int j = 0; j < PT; ++j) dst[(half0 + j) * 64 + lane] = v[j];
+        }
+    };
+    uint2 sv[SV][PS];
+    auto load_scales = [&](int q, uint2 *v) {   // of a pair of spans
+#pragma unroll
+        for (int j = 0; j < PS; ++j) v[j] = *reinterpret_cast<const uint2 *>(sr[j] + (size_t)min(2 * q + odd_thread, last) * 8);
+    };
+    auto store_scales = [&](const uint2 *v, uint16_t *dst) {
+#pragma unroll
+        for (int j = 0; j < PS; ++j) *reinterpret_cast<uint2 *>(&dst[(j * 256 + threadIdx.x) % (2 * TM) * 4]) = v[j];
+    };
+    auto arrived = [&] {   // what the waves put into LDS is there
+        if constexpr (PF == 1) {
+            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+            __syncthreads();
+        } else {
+            // Without __syncthreads()'s wait for the loads under way. Matrix instructions may move past, memory's may not.
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0x8);
+        }
+    };
+    v4i *const xt[2] = {xt0, xt1};
+    uint16_t *const xs[2] = {xs0, xs1};
+#pragma unroll
+    for (int q = 0; q < SV; ++q) load_scales(min(q, last / 2), sv[q]);
+#pragma unroll
+    for (int k = 0; k < PF; ++k) load_rows(min(k, last), xv[k], xt[k & 1]);
+
+    v4f acc[RT][TT] = {};
+    // where a piece lies that this lane reads: row n's 2 slot and 2 slot + 1
+    const int at0 = 64 * (n >> 3) + 8 * (n & 7) + ((2 * slot) ^ (n >> 1)), at1 = at0 ^ 1;
+    // The span p = K modulo 4. What goes out here is for the span p + PF (near the end: the last one, again. Without a
+    // branch, so that the compiler knows how many loads are under way and waits for the older ones alone).
+    auto span = [&](auto k, int p) {
+        constexpr int K = decltype(k)::value, H = K & 1, Q = K >> 1, B = K % R, N = (K + PF) % R;
+        if (H == 0) load_scales(min(p / 2 + SV, last / 2), sv[Q % SV]);
+        load_rows(min(p + PF, last), xv[N], xt[N & 1]);
+        load_weights(min(p + PF, last), w[N]);
+        __builtin_amdgcn_sched_barrier(0);   // where the loads stand is where they go out
+        v4i b[2][2];
+        uint32_t sx[2];
+        auto read = [&](int t) {
+            b[t & 1][0] = xt[H][t * 128 + at0];
+            b[t & 1][1] = xt[H][t * 128 + at1];
+            sx[t & 1] = xs[Q][(n * 2 + H) * 4 + slot + t * 128];
+        };
+        read(0);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            if (t + 1 < TT) read(t + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                acc[i][t] = span_mfma<H>(acc[i][t], w[B].c[i][0], w[B].c[i][1], w[B].s[i], b[t & 1][0], b[t & 1][1], sx[t & 1]);
+        }
+        store_rows(xv[(K + 1) % R], xt[H ^ 1]);
+        if (H == 1) store_scales(sv[(Q + 1) % SV], xs[Q ^ 1]);
+        arrived();
+    };
+    store_rows(xv[0], xt0);
+    store_scales(sv[0], xs0);
+    arrived();
+    auto pair = [&](auto q, int p) {
+        constexpr int Q = decltype(q)::value;
+        span(std::integral_constant<int, 2 * Q>{}, p);
+        if (p == last) return;
+        span(std::integral_constant<int, 2 * Q + 1>{}, p + 1);
+    };
+    for (int p = 0; p <= last; p += 4) {
+        pair(std::integral_constant<int, 0>{}, p);
+        if (p + 2 <= last) pair(std::integral_constant<int, 1>{}, p + 2);
+    }
+
+    bool ok[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const int m = lo + 16 * t + n;
+        ok[t] = m < hi;
+        if (GROUPED) {
+            const int c = min(m, hi - 1), r = a.index ? a.index[c] : c;
+            ok[t] = ok[t] && r >= 0 && r < a.rows_in;
         }
     }
+    const int out_rows = GLU ? a.rows / 2 : a.rows, tile0 = (rb * 4 + wave) * OT;
+    if (tile0 >= otiles) return;
+    float b0[OT][4] = {}, b1[OT][4] = {};
+    if (a.bias) {
+        const float *bias = a.bias + (size_t)expert * a.rows;
 #pragma unroll
-    for (int h = 0; h < NT; ++h) red[wave][h][lane] = acc[h];
-    __syncthreads();
-    if (wave != 0 || n >= a.M) return;
-    const int out_rows = GLU ? a.rows / 2 : a.rows;
-    v4f s[NT];
-#pragma unroll
-    for (int h = 0; h < NT; ++h) s[h] = ((red[0][h][lane] + red[1][h][lane]) + red[2][h][lane]) + red[3][h][lane];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = tile * 16 + slot * 4 + i;
-        if (r >= out_rows) continue;
-        float v = s[0][i] + (a.bias ? a.bias[r] : 0.0f);
-        if (GLU) v = swiglu(v, s[NT - 1][i] + (a.bias ? a.bias[out_rows + r] : 0.0f));
-        a.y[(int64_t)n * a.ldy + r] = v;
+        for (int i = 0; i < OT; ++i) load_bias<GLU>(bias, (tile0 + i) * 16 + slot * 4, out_rows, b0[i], b1[i]);
     }
+    auto store = [&](auto whole) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            if (!ok[t]) continue;
+            float *yr = a.y + (int64_t)(lo + 16 * t + n) * a.ldy;
+#pragma unroll
+            for (int i = 0; i < OT; ++i)
+                store_outputs<GLU, decltype(whole)::value>(yr, (tile0 + i) * 16 + slot * 4, out_rows, acc[i][t], acc[RT - OT + i][t],
+                                                        b0[i], b1[i]);
+        }
+    };
+    if (a.vec && (tile0 + OT) * 16 <= out_rows)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
 }
 
 // ---- host ----
 
-constexpr int kMaxCols = 1 << 30;
+constexpr int kMaxCols = 1 << 24;
+constexpr int kMaxRows = 1 << 30;
+constexpr int kTilesBehind = 15;   // row tiles that a product may read behind the last
 constexpr int kRowsMaxM = 8, kRowsMaxCols = 16384;
 
 inline int spans_of(int cols) { return (cols - 1) / kSpan + 1; }
@@ -413,7 +689,7 @@ int launch_quant(const void *x, int64_t ldx, int rows, int cols, uint8_t *codes,
     const int64_t blocks = ((int64_t)rows * spans + 3) / 4;
     if (blocks > INT32_MAX) return EIF_HIP_E_LIMIT;
     const T *xt = static_cast<const T *>(x);
-    if (aligned(x, 4 * sizeof(T)) && ldx % 4 == 0)
+    if (aligned(x, 4 * sizeof(T)) && ldx % 4 == 0 && cols % 4 == 0)
         quant_rows_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv);
     else
         quant_rows_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv);
@@ -444,34 +720,114 @@ Mx4Args weight_args(const eif_hip_mx4_weight *w, const float *bias, float *y, in
     Mx4Args a{};
     a.wc = w->codes, a.ws = w->scales, a.tiles = w->tiles, a.spans = w->spans, a.rows = w->rows, a.cols = w->cols;
     a.bias = bias, a.y = y, a.ldy = ldy, a.M = M, a.experts = w->experts;
+    a.vec = aligned(y, 16) && ldy % 4 == 0;
     return a;
 }
 
-template <int TT>
-int launch_linear(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
+// Groups of `per` token rows: what the grid holds (by expert: however the rows are spread), and about how many there are.
+struct Groups {
+    int64_t grid, likely;
+};
+Groups groups_of(const Mx4Args &a, bool grouped, int per)
 {
-    const int64_t groups = (int64_t)(a.M - 1) / (16 * TT) + 1 + (grouped ? a.experts - 1 : 0);
-    const int64_t blocks = groups * (glu ? a.tiles / 2 : a.tiles);
+    const int64_t whole = (int64_t)(a.M - 1) / per + 1;
+    if (!grouped) return {whole, whole};
+    return {whole + a.experts - 1, std::min<int64_t>(whole + a.experts / 2, a.M)};
+}
+
+template <typename X, int TT, int KW, int D>
+int launch_split_as(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
+{
+    const int64_t blocks = groups_of(a, grouped, 16 * TT).grid * eif_ceil_div(glu ? a.tiles / 2 : a.tiles, 8 / KW);
     if (blocks > INT32_MAX) return EIF_HIP_E_LIMIT;
     const unsigned g = (unsigned)blocks;
-    if (glu)
-        grouped ? mx4_linear_kernel<TT, true, true><<<g, 256, 0, st>>>(a) : mx4_linear_kernel<TT, true, false><<<g, 256, 0, st>>>(a);
-    else
-        grouped ? mx4_linear_kernel<TT, false, true><<<g, 256, 0, st>>>(a) : mx4_linear_kernel<TT, false, false><<<g, 256, 0, st>>>(a);
+    if constexpr (std::is_void<X>::value) {
+        if (glu)
+            grouped ? mx4_split_kernel<X, TT, KW, D, true, true><<<g, 512, 0, st>>>(a)
+                    : mx4_split_kernel<X, TT, KW, D, true, false><<<g, 512, 0, st>>>(a);
+        else
+            grouped ? mx4_split_kernel<X, TT, KW, D, false, true><<<g, 512, 0, st>>>(a)
+                    : mx4_split_kernel<X, TT, KW, D, false, false><<<g, 512, 0, st>>>(a);
+    } else {
+        const size_t lds = (size_t)a.M * (a.spans * 128 + 16 + a.spans * 8);
+        if (glu)
+            mx4_split_kernel<X, TT, KW, D, true, false><<<g, 512, lds, st>>>(a);
+        else
+            mx4_split_kernel<X, TT, KW, D, false, false><<<g, 512, lds, st>>>(a);
+    }
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
 
-template <typename T>
-int launch_rows(const Mx4Args &a, bool glu, hipStream_t st)
+template <typename X, int TT, int KW>
+int launch_split_deep(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
-    const size_t lds = (size_t)a.M * (a.spans * 128 + 16 + a.spans * 8);
+    const int n = eif_ceil_div(a.spans, KW);   // spans of a wave
+    if (n == 1) return launch_split_as<X, TT, KW, 1>(a, glu, grouped, st);
+    if (n == 2 || TT > 1) return launch_split_as<X, TT, KW, 2>(a, glu, grouped, st);
+    return launch_split_as<X, TT, KW, TT == 1 ? 4 : 2>(a, glu, grouped, st);
+}
+
+// Waves that share a row tile: as many as keep the launch at 4096 waves, 4 a SIMD (the rows form: 2048; each workgroup
+// quantises the rows, and more waves a tile are more workgroups). Measured (us, 1 / 2 / 4 / 8 waves): one row, 151936x1024
+// 13.9 / 14.1 / 15.2 / 23.1; 8 rows, 8192x8192 19.8 / 11.9 / 9.2 / 8.7, gated 13824x2560 in the rows form 11.0 / 9.8 /
+// 9.2 / 11.0; 32 rows by expert, about 22 experts of gated 2816x2560 13.6 / 18.1 / 19.4 / 17.2.
+template <typename X, int TT>
+int launch_split(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
+{
+    const int64_t tiles = groups_of(a, grouped, 16 * TT).likely * (glu ? a.tiles / 2 : a.tiles);
+    const int64_t waves = std::is_void<X>::value ? 4096 : 2048;
+    int kw = 8;
+    while (kw > 1 && (kw > a.spans || tiles * kw > waves)) kw /= 2;
+    if (kw == 8) return launch_split_deep<X, TT, 8>(a, glu, grouped, st);
+    if (kw == 4) return launch_split_deep<X, TT, 4>(a, glu, grouped, st);
+    if (kw == 2) return launch_split_deep<X, TT, 2>(a, glu, grouped, st);
+    return launch_split_deep<X, TT, 1>(a, glu, grouped, st);
+}
+
+// Workgroups of mx4_gemm_kernel<RT, TT>: row blocks times groups.
+template <int RT, int TT>
+int64_t gemm_blocks(const Mx4Args &a, bool glu, int64_t groups)
+{
+    return groups * eif_ceil_div(glu ? a.tiles / 2 : a.tiles, 4 * RT / (glu ? 2 : 1));
+}
+
+template <int RT, int TT, int PF>
+int launch_gemm(Mx4Args a, bool glu, bool grouped, hipStream_t st)
+{
+    const int64_t groups = groups_of(a, grouped, 16 * TT).grid, blocks = gemm_blocks<RT, TT>(a, glu, groups);
+    if (blocks > (1 << 28)) return EIF_HIP_E_LIMIT;
+    a.groups = (int)groups;
+    const unsigned g = (unsigned)(blocks + 7) / 8 * 8;
     if (glu)
-        mx4_rows_kernel<T, true><<<a.tiles / 2, 256, lds, st>>>(a);
+        grouped ? mx4_gemm_kernel<RT, TT, PF, true, true><<<g, 256, 0, st>>>(a)
+                : mx4_gemm_kernel<RT, TT, PF, true, false><<<g, 256, 0, st>>>(a);
     else
-        mx4_rows_kernel<T, false><<<a.tiles, 256, lds, st>>>(a);
+        grouped ? mx4_gemm_kernel<RT, TT, PF, false, true><<<g, 256, 0, st>>>(a)
+                : mx4_gemm_kernel<RT, TT, PF, false, false><<<g, 256, 0, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
+}
+
+// The form of a product of quantised rows: the largest tile that still gives the CUs (256) workgroups enough, 1.5 each or
+// more; of a few rows the split form. By expert a tile of more token rows than an expert has on average is mostly empty.
+// Measured (us; 256 rows x 128 tokens / 128x128 / 128x64 / 128x32 three spans ahead / split):
+//   4096 rows, 8192x8192 151 / 173 / 218 / 325 / -; 512, gated 13824x2560 17.8 / 16.7 / 18.9 / 24.4 / 55
+//   1024, 4096x4096 24.4 / 17.4 / 16.4 / 22.4 / -; 256, 2560x6912 34 / 23.4 / 19.1 / 12.2 / 25; 128, 8192x8192 38 / 26 / 21 /
+//   13.9 / 50; 100, 2560x2560 14.8 / 9.9 / 7.1 / 6.5 / 8.0; 48, 4864x896 - / 5.5 / 4.5 / 4.3 / 3.6; 24, 2560x6912 - / 18.6 /
+//   16.8 / 16 / 6.1; by expert, gated 2816 rows: 16384 rows to 64 103 / 112 / 119 / 160 / -, 800 to 32 35 / 37 / 31 / 35 / 42.
+int launch_product(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
+{
+    const int m = grouped ? (a.M - 1) / a.experts + 1 : a.M;   // token rows of a matrix
+    const int64_t enough = 384;
+    if (m <= 16) return launch_split<void, 1>(a, glu, grouped, st);
+    const int64_t g128 = groups_of(a, grouped, 128).likely, g64 = groups_of(a, grouped, 64).likely;
+    if (m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= enough) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
+    if (m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= enough) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
+    if (gemm_blocks<2, 4>(a, glu, g64) >= enough) return launch_gemm<2, 4, 1>(a, glu, grouped, st);
+    if (a.spans >= 8 && gemm_blocks<2, 2>(a, glu, groups_of(a, grouped, 32).likely) >= 64)
+        return launch_gemm<2, 2, 3>(a, glu, grouped, st);
+    return m <= 32 ? launch_split<void, 2>(a, glu, grouped, st) : launch_split<void, 1>(a, glu, grouped, st);
 }
 
 }  // namespace
@@ -505,7 +861,7 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     *out = nullptr;
     if (!codes || !scales || experts < 1 || rows < 1 || cols < 1) return EIF_HIP_E_ARG;
     if (ldc < ((int64_t)cols + 1) / 2 || lds < ((int64_t)cols + 31) / 32) return EIF_HIP_E_ARG;
-    if (cols > kMaxCols || rows > kMaxCols) return EIF_HIP_E_LIMIT;
+    if (cols > kMaxCols || rows > kMaxRows) return EIF_HIP_E_LIMIT;
     eif_hip_mx4_weight q{};
     q.experts = experts, q.rows = rows, q.cols = cols, q.tiles = eif_ceil_div(rows, 16), q.spans = spans_of(cols);
     if ((int64_t)experts * q.tiles > INT32_MAX) return EIF_HIP_E_LIMIT;
@@ -520,7 +876,8 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     const size_t src_c = (all - 1) * ldc + ((size_t)cols + 1) / 2, src_s = (all - 1) * lds + ((size_t)cols + 31) / 32;
     uint8_t *up = nullptr;
     int rc = EIF_HIP_OK;
-    if (hipMalloc(&q.codes, cbytes) != hipSuccess || hipMalloc(&q.scales, sdwords * 4) != hipSuccess ||
+    if (hipMalloc(&q.codes, cbytes + kTilesBehind * tile_codes(q.spans)) != hipSuccess ||
+        hipMalloc(&q.scales, (sdwords + kTilesBehind * tile_scales(q.spans)) * 4) != hipSuccess ||
         (!src_on_device && hipMalloc(&up, src_c + src_s) != hipSuccess)) {
         (void)hipGetLastError();
         rc = EIF_HIP_E_NOMEM;
@@ -541,7 +898,7 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     }
     if (rc != EIF_HIP_E_NOMEM && hipStreamSynchronize(st) != hipSuccess && rc == EIF_HIP_OK) rc = EIF_HIP_E_DEVICE;
     if (up) (void)hipFree(up);
-    q.bytes = cbytes + sdwords * 4;
+    q.bytes = cbytes + sdwords * 4 + kTilesBehind * (tile_codes(q.spans) + tile_scales(q.spans) * 4);
     eif_hip_mx4_weight *h = rc == EIF_HIP_OK ? new (std::nothrow) eif_hip_mx4_weight(q) : nullptr;
     if (!h) {
         if (q.codes) (void)hipFree(q.codes);
@@ -581,7 +938,7 @@ int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_
     if ((rc = check_operand(w, codes, ldc, scales, lds)) != 0) return rc;
     Mx4Args a = weight_args(w, bias, y, ldy, M);
     a.codes = codes, a.ldc = ldc, a.scales = scales, a.lds = lds;
-    return M <= 16 ? launch_linear<1>(a, glu, false, (hipStream_t)stream) : launch_linear<4>(a, glu, false, (hipStream_t)stream);
+    return launch_product(a, glu, false, (hipStream_t)stream);
 }
 
 int eif_hip_mx4_linear_rows(const eif_hip_mx4_weight *w, const void *x, int type, int64_t ldx, const float *bias, int glu,
@@ -596,8 +953,9 @@ int eif_hip_mx4_linear_rows(const eif_hip_mx4_weight *w, const void *x, int type
     Mx4Args a = weight_args(w, bias, y, ldy, M);
     a.x = x, a.ldx = ldx;
     hipStream_t st = (hipStream_t)stream;
-    if (type == EIF_HIP_F32) return launch_rows<float>(a, glu, st);
-    return type == EIF_HIP_F16 ? launch_rows<__half>(a, glu, st) : launch_rows<__hip_bfloat16>(a, glu, st);
+    a.vecx = aligned(x, type == EIF_HIP_F32 ? 16 : 8) && ldx % 4 == 0 && w->cols % 4 == 0;
+    if (type == EIF_HIP_F32) return launch_split<float, 1>(a, glu, false, st);
+    return type == EIF_HIP_F16 ? launch_split<__half, 1>(a, glu, false, st) : launch_split<__hip_bfloat16, 1>(a, glu, false, st);
 }
 
 int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales,
@@ -613,8 +971,7 @@ int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes
     Mx4Args a = weight_args(w, bias, y, ldy, M);
     a.codes = codes, a.ldc = ldc, a.scales = scales, a.lds = lds;
     a.rows_in = rows_in, a.index = row_index, a.offsets = offsets;
-    return M <= 16 * (int64_t)w->experts ? launch_linear<1>(a, glu, true, (hipStream_t)stream)
-                                         : launch_linear<4>(a, glu, true, (hipStream_t)stream);
+    return launch_product(a, glu, true, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -29,7 +29,7 @@ extern "C" {
 /* Element types of rows. */
 enum { EIF_HIP_F32 = 0, EIF_HIP_F16 = 1, EIF_HIP_BF16 = 2 };
 
-/* Columns of an operand row of the products: cols rounded up to a multiple of 256 (0 for cols < 1 or beyond 2^30). */
+/* Columns of an operand row of the products: cols rounded up to a multiple of 256 (0 for cols < 1 or beyond 2^24). */
 int eif_hip_mx4_kpad(int cols);
 
 /* Rows x [rows, ldx] of `type` -> MXFP4. Per block: a = the largest magnitude; b = max(0, floor(log2 a) + 125), 0 where

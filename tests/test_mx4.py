@@ -56,7 +56,7 @@ def test_quant_refuses(fake):  # noqa: F811
                 dict(x=at(2)), dict(type=1, x=at(1)), dict(cols=257, ldx=257, ldv=257)):
         assert q(**bad) == ARG, bad
     assert q(type=1, x=at(2)) == 0 and q(x=at(4)) == 0
-    big = 1 << 30
+    big = 1 << 24
     assert q(cols=big + 1, ldx=big + 1, ldc=big, lds=big, ldv=big + 1) == LIMIT
     assert q(rows=1 << 30, cols=1 << 20, ldx=1 << 20, ldc=1 << 19, lds=1 << 15, ldv=1 << 20) == LIMIT
     fake.fake_reset(); fake.fake_fail_launch(0)
@@ -79,7 +79,7 @@ def test_create_refuses_and_gives_back(fake):  # noqa: F811
                 dict(lds=1), dict(cols=65, ldc=32), dict(cols=65, ldc=33)):
         assert create(**bad) == ARG, bad
     assert create(cols=65, ldc=33, lds=3) == 0
-    assert create(rows=(1 << 30) + 1) == LIMIT and create(experts=1 << 20, rows=1 << 20) == LIMIT
+    assert create(rows=(1 << 30) + 1) == LIMIT and create(cols=(1 << 24) + 1, ldc=1 << 24, lds=1 << 20) == LIMIT and create(experts=1 << 20, rows=1 << 20) == LIMIT
     for dev in (0, 1):
         fake.fake_reset(); fake.fake_fail_malloc(1)
         assert create(dev=dev) == -3 and fake.fake_live() == 0
@@ -90,7 +90,7 @@ def test_create_refuses_and_gives_back(fake):  # noqa: F811
     w = mx4(33, 300, 3)
     i = [C.c_int() for _ in range(4)]; b = C.c_size_t()
     assert lib.eif_hip_mx4_weight_info(w.h, *map(C.byref, i), C.byref(b)) == 0 and [v.value for v in i] == [3, 33, 300, 512]
-    assert b.value == 9 * (2 * 2048 + 256) and lib.eif_hip_mx4_weight_info(None, None, None, None, None, None) == ARG
+    assert b.value == (9 + 15) * (2 * 2048 + 256)   # 15 row tiles behind the last and lib.eif_hip_mx4_weight_info(None, None, None, None, None, None) == ARG
     w.close(); w.close(); lib.eif_hip_mx4_weight_destroy(None)
     assert fake.fake_live() == 0
     """)
