@@ -106,20 +106,21 @@ EIF_DEV uint32_t quantise4(const float *v, uint32_t &byte)
     return codes4(v, scale_inverse(byte), byte != 255);
 }
 
-// One wave a row and span: lane l has columns 4 l .. 4 l + 3, a block is eight lanes.
+// One wave a row and span: lane l has columns 4 l .. 4 l + 3, a block is eight lanes, and a wave's loads and stores are one run.
+// Bound by memory: 3001x6912 FP32 with values 34.3 us, 5.2 TB/s of what it reads and writes (43 with values stored four bytes at
+// a time); without values 17.7, 5.3 TB/s. Two to eight spans a wave, their loads first, were no faster (34.0 to 37.6) and small
+// calls slower (64x2560 2.1 us with one, 2.5 with two).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx, int rows, int cols, int spans,
                                                          uint8_t *codes, int64_t ldc, uint8_t *scales, int64_t lds,
-                                                         float *values, int64_t ldv)
+                                                         float *values, int64_t ldv, bool vec_values)
 {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t row = unit / spans;
-    const int span = (int)(unit % spans), c = span * kSpan + lane * 4;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = unit / spans;
     if (row >= rows) return;
-    const T *xr = x + row * ldx;
+    const int c = (int)(unit - row * spans) * kSpan + lane * 4;
     float v[4];
-    values4(load4<T, VEC>(xr, c, cols), c, cols, v);
+    values4(load4<T, VEC>(x + row * ldx, c, cols), c, cols, v);
     uint32_t b;
     const uint32_t q = quantise4(v, b);
     if (codes) {
@@ -131,10 +132,14 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx
         const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0);
         const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
         const float o[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
-        float *vr = values + row * ldv;
+        float *vr = values + row * ldv + c;
+        if (vec_values && c + 4 <= cols) {
+            *reinterpret_cast<float4 *>(vr) = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < cols) vr[c + i] = o[i];
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) vr[i] = o[i];
+        }
     }
 }
 
@@ -688,11 +693,12 @@ int launch_quant(const void *x, int64_t ldx, int rows, int cols, uint8_t *codes,
     const int spans = spans_of(cols);
     const int64_t blocks = ((int64_t)rows * spans + 3) / 4;
     if (blocks > INT32_MAX) return EIF_HIP_E_LIMIT;
+    const bool vv = aligned(values, 16) && ldv % 4 == 0;
     const T *xt = static_cast<const T *>(x);
     if (aligned(x, 4 * sizeof(T)) && ldx % 4 == 0 && cols % 4 == 0)
-        quant_rows_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv);
+        quant_rows_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv, vv);
     else
-        quant_rows_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv);
+        quant_rows_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv, vv);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
@@ -768,15 +774,15 @@ int launch_split_deep(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
     return launch_split_as<X, TT, KW, TT == 1 ? 4 : 2>(a, glu, grouped, st);
 }
 
-// Waves that share a row tile: as many as keep the launch at 4096 waves, 4 a SIMD (the rows form: 2048; each workgroup
-// quantises the rows, and more waves a tile are more workgroups). Measured (us, 1 / 2 / 4 / 8 waves): one row, 151936x1024
+// Waves that share a row tile: as many as keep the launch at 4096 row tiles times waves, 4 a SIMD (the rows form: 3500; each
+// workgroup quantises the rows, and more waves a tile are more workgroups). Measured (us, 1 / 2 / 4 / 8 waves): one row, 151936x1024
 // 13.9 / 14.1 / 15.2 / 23.1; 8 rows, 8192x8192 19.8 / 11.9 / 9.2 / 8.7, gated 13824x2560 in the rows form 11.0 / 9.8 /
 // 9.2 / 11.0; 32 rows by expert, about 22 experts of gated 2816x2560 13.6 / 18.1 / 19.4 / 17.2.
 template <typename X, int TT>
 int launch_split(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
-    const int64_t tiles = groups_of(a, grouped, 16 * TT).likely * (glu ? a.tiles / 2 : a.tiles);
-    const int64_t waves = std::is_void<X>::value ? 4096 : 2048;
+    const int64_t tiles = groups_of(a, grouped, 16 * TT).likely * a.tiles;
+    const int64_t waves = std::is_void<X>::value ? 4096 : 3500;
     int kw = 8;
     while (kw > 1 && (kw > a.spans || tiles * kw > waves)) kw /= 2;
     if (kw == 8) return launch_split_deep<X, TT, 8>(a, glu, grouped, st);
