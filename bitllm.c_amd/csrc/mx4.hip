@@ -235,7 +235,8 @@ EIF_DEV float swiglu(float g, float u)
 }
 
 // The g-th group of TM token rows over the experts' ranges: its expert and its rows [lo, hi); false beyond the last.
-// One wave's lanes take 64 experts at a time; a range is cut to [0, M], so every row is in bounds whatever the offsets.
+// One wave's lanes take 64 experts at a time; a range is cut to [0, M], and a group taken only inside its range, so every
+// row is in bounds whatever the offsets.
 template <int TM>
 EIF_DEV bool find_group(const Mx4Args &a, int g, int &expert, int &lo, int &hi)
 {
@@ -260,6 +261,7 @@ EIF_DEV bool find_group(const Mx4Args &a, int g, int &expert, int &lo, int &hi)
             const int l = __ffsll(past) - 1;
             const int at = g - (base + __shfl(sum - groups, l, 64));
             const int s0 = __shfl(s, l, 64), n0 = __shfl(n, l, 64);
+            if (at < 0 || at >= (n0 + TM - 1) / TM) return false;   // ranges that overlap, with sums beyond an int
             expert = __builtin_amdgcn_readfirstlane(e0 + l);
             lo = __builtin_amdgcn_readfirstlane(s0 + at * TM);
             hi = __builtin_amdgcn_readfirstlane(min(s0 + at * TM + TM, s0 + n0));
@@ -707,6 +709,7 @@ int launch_quant(const void *x, int64_t ldx, int rows, int cols, uint8_t *codes,
 int check_product(const eif_hip_mx4_weight *w, int glu, const float *y, int64_t ldy, int M)
 {
     if (!w || M < 0) return EIF_HIP_E_ARG;
+    if (M > kMaxRows) return EIF_HIP_E_LIMIT;
     if (glu && w->rows % 32 != 0) return EIF_HIP_E_LIMIT;
     if (ldy < (glu ? w->rows / 2 : w->rows) || (M > 0 && !y)) return EIF_HIP_E_ARG;
     int dev = -1;

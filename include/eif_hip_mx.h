@@ -59,8 +59,9 @@ int eif_hip_mx4_weight_info(const eif_hip_mx4_weight *w, int *experts, int *rows
  * in an order that depends on the shapes alone. Sums below the smallest normal number may come out as 0, and a sum whose
  * partial sums leave FP32's range as an infinity or NaN.
  * glu != 0: the matrix stacks gate rows (0 .. rows/2 - 1) over up rows (rows/2 .. rows - 1); y [M, rows/2] =
- * SiLU(g) u = (g * (1 / (1 + expf(-g)))) * u of the two products with their biases; rows a multiple of 32, else
- * EIF_HIP_E_LIMIT.                                                                                           */
+ * SiLU(g) u = (g / (1 + e^-g)) u of the two products with their biases, the exponential and the quotient with the GPU's own
+ * instructions (beside the rounding of g, 2^-21 of the result). rows a multiple of 32, else EIF_HIP_E_LIMIT.
+ * M beyond 2^30, and products of more workgroups than a launch holds (2^28): EIF_HIP_E_LIMIT.               */
 int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales, int64_t lds,
                        const float *bias, int glu, float *y, int64_t ldy, int M, void *stream);
 
@@ -74,7 +75,8 @@ int eif_hip_mx4_linear_rows(const eif_hip_mx4_weight *w, const void *x, int type
  * [experts, rows] or NULL, and glu as above). offsets [experts + 1] int32 in device memory, non-decreasing, taken as if
  * cut to [0, M]; experts may have no rows. Row i of y takes the quantised row row_index[i] (int32 in device memory; NULL:
  * i) of `rows_in` rows. Rows of y before offsets[0] and from offsets[experts] on, and rows whose index is not in
- * [0, rows_in), are left as they were. (Offsets that decrease leave it open which rows are written.) */
+ * [0, rows_in), are left as they were. (Where offsets decrease, so that ranges overlap, it is open which
+ * of their rows are written, and with whose products.) */
 int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales,
                                int64_t lds, int rows_in, const int32_t *row_index, const int32_t *offsets,
                                const float *bias, int glu, float *y, int64_t ldy, int M, void *stream);

@@ -315,6 +315,154 @@ def test_grouped_offsets_cut(gpu):
         check(y, *grouped_want(c, np.clip(offsets.astype(np.int64), 0, m), None, m, n, False, None))
 
 
+LARGE = [  # rows, token rows: the tiles of 256x128, 128x128, 128x64 and 128x32 (rows x token rows)
+    (4130, 3070), (9920, 600), (2880, 1101), (1100, 300)]
+
+
+def large(gpu, n, k, m, experts=1):
+    """A weight, operand rows and biases made on the GPU, and their values in 64 bits there."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(n + k + m)
+
+    def packed(rows, scale):
+        x = torch.randn((rows, k), device="cuda", generator=g) * scale
+        c, s, v = rows_on_gpu(gpu, x * torch.exp2(torch.randn((rows, 1), device="cuda", generator=g)))
+        return c, s, v.double()
+
+    wc, ws, wv = packed(experts * n, k ** -0.5)
+    w = gpu.Mx4Weight(n, k, wc, ws, experts=experts)
+    ac, as_, av = packed(m, 1.0)
+    return w, wv.reshape(experts, n, k), ac, as_, av, torch.randn((experts, n), device="cuda", generator=g)
+
+
+def product_on_gpu(a, w, bias, glu):
+    """mx4_ref.product on GPU tensors."""
+    import torch
+    k = a.shape[1]
+    y = a @ w.T + bias.double()
+    tol = (-(-k // 32) + 16) * 2.0 ** -23 * (a.abs() @ w.abs().T) + 2.0 ** -126 + 2.0 ** -23 * (y.abs() + bias.double().abs())
+    if not glu:
+        return y, tol
+    (g, u), (tg, tu) = y.chunk(2, 1), tol.chunk(2, 1)
+    silu = g * torch.sigmoid(g)
+    return silu * u, 1.1 * tg * (u.abs() + tu) + (silu.abs() + 1.1 * tg) * tu + 2.0 ** -21 * (silu * u).abs() + 2.0 ** -126
+
+
+def check_on_gpu(y, want, tol):
+    bad = ~((y.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("n,m", LARGE)
+@pytest.mark.parametrize("k", [256, 300, 700, 1024, 1300, 2304])
+@pytest.mark.parametrize("glu", [False, True])
+def test_linear_large(gpu, n, m, k, glu):
+    import torch
+    n = -(-2 * n // 32) * 32 if glu else n
+    w, wv, ac, as_, av, bias = large(gpu, n, k, m)
+    want, tol = product_on_gpu(av, wv[0], bias[0], glu)
+    cols = n // 2 if glu else n
+    for pad in (0, 3):   # rows of y whose 16-byte stores are whole, and others
+        y = torch.full((m, cols + pad), float("nan"), device="cuda")[:, :cols]
+        w.linear(ac, as_, y, bias[0], glu=glu)
+        check_on_gpu(y, want, tol)
+
+
+@pytest.mark.parametrize("n,m,experts", [(2304, 6000, 7), (1536, 3000, 20), (640, 4000, 40), (1100, 700, 9)])
+@pytest.mark.parametrize("k", [300, 1536])
+@pytest.mark.parametrize("glu", [False, True])
+def test_grouped_large(gpu, n, m, experts, k, glu):
+    import torch
+    n = -(-2 * n // 32) * 32 if glu else n
+    t = m // 3
+    w, wv, ac, as_, av, bias = large(gpu, n, k, t, experts)
+    rng = np.random.default_rng(m)
+    offsets = np.concatenate([[0], np.cumsum(spread(rng, m - 5, experts, "ragged"))]).astype(np.int32) + 2
+    idx = rng.integers(0, t, m).astype(np.int32)
+    idx[::11] = -1
+    y = torch.full((m, n // 2 if glu else n), float("nan"), device="cuda")
+    w.linear_grouped(ac, as_, dev(offsets), y, dev(idx), bias, glu)
+    left = np.ones(m, bool)
+    for e in range(experts):
+        rows = np.arange(offsets[e], offsets[e + 1])
+        rows = rows[idx[rows] >= 0]
+        left[rows] = False
+        if len(rows):
+            at = torch.from_numpy(rows).cuda()
+            check_on_gpu(y[at], *product_on_gpu(av[torch.from_numpy(idx[rows]).cuda().long()], wv[e], bias[e], glu))
+    assert y[torch.from_numpy(left).cuda()].isnan().all()
+
+
+def test_grouped_offsets_in_any_order(gpu):
+    """Offsets that decrease or ranges that overlap: every output written is that of some expert whose range holds it."""
+    import torch
+    experts, n, k, m = 70, 32, 256, 200
+    c = Case(gpu, 4, n, k, m, experts=experts)
+    rng = np.random.default_rng(8)
+    for offsets in (rng.integers(-50, 300, experts + 1), np.tile([0, m], 36)[:experts + 1], np.arange(experts, -1, -1)):
+        offsets = offsets.astype(np.int32)
+        y = out(m, n)
+        c.w.linear_grouped(c.ac, c.as_, dev(offsets), y)
+        torch.cuda.synchronize()
+        got = host(y).astype(np.float64)
+        fits = np.isnan(got)
+        for e in range(experts):
+            rows = np.arange(max(offsets[e], 0), min(max(offsets[e + 1], 0), m))
+            want, tol = mx4_ref.product(c.av[rows], c.wv[e])
+            fits[rows] |= np.abs(got[rows] - want) <= tol
+        assert fits.all()
+
+
+FAR = [(1, 40), (3, 40), (40, 40), (300, 40)]   # token rows, rows
+
+
+@pytest.mark.parametrize("m,n", FAR)
+def test_offsets_beyond_32_bits(gpu, m, n):
+    """Rows so far apart that the last ones lie behind 2^32 bytes: operands, outputs, the quantiser's inputs and outputs."""
+    import torch
+    k = 300
+    c = Case(gpu, m, n, k, m)
+    far = (5 << 30) // max(m - 1, 1) // 16 * 16 + 1024
+    codes = torch.empty(far * (m - 1) + 4096, dtype=torch.uint8, device="cuda").as_strided((m, 256), (far, 1))
+    scales = torch.empty(far * (m - 1) + 4096, dtype=torch.uint8, device="cuda").as_strided((m, 16), (far, 1))
+    x = torch.empty(far // 4 * (m - 1) + 4096, device="cuda").as_strided((m, k), (far // 4, 1))
+    y = torch.empty(far // 4 * (m - 1) + 4096, device="cuda").as_strided((m, n), (far // 4, 1))
+    x.copy_(dev(c.a))
+    y.fill_(float("nan"))
+    gpu.mx4_quant_rows(x, codes, scales)
+    assert torch.equal(codes, c.ac) and torch.equal(scales, c.as_)
+    want = mx4_ref.product(c.av, c.wv[0])
+    c.w.linear(codes, scales, y)
+    check(y, *want)
+    y.fill_(float("nan"))
+    c.w.linear_grouped(codes, scales, dev(np.array([0, m], np.int32)), y)
+    check(y, *want)
+    if m <= 8:
+        y.fill_(float("nan"))
+        c.w.linear_rows(x, y)
+        check(y, *want)
+
+
+@pytest.mark.parametrize("m", [3, 60, 200])
+def test_stack_beyond_32_bits(gpu, m):
+    """A stack of matrices of more than 2^32 bytes: the last one's products, at some of its rows."""
+    import torch
+    experts, n, k = 5, 65536, 32768
+    g = torch.Generator(device="cuda").manual_seed(m)
+    wc = torch.randint(0, 256, (experts, n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    ws = torch.randint(120, 126, (experts, n, k // 32), dtype=torch.uint8, device="cuda", generator=g)
+    w = gpu.Mx4Weight(n, k, wc, ws, experts=experts)
+    assert w.bytes > 1 << 32
+    ac, as_ = mx4_ref.quantise(mx4_ref.activations(np.random.default_rng(m), m, k))
+    y = out(m, n)
+    w.linear_grouped(dev(ac), dev(as_), dev(np.array([0, 0, 0, 0, 0, m], np.int32)), y)
+    torch.cuda.synchronize()
+    assert not y.isnan().any()
+    at = [0, 1, 17, 32767, 40000, 65520, 65535]
+    want, tol = mx4_ref.product(mx4_ref.values(ac, as_, k), mx4_ref.values(host(wc[4, at]), host(ws[4, at]), k))
+    check(y[:, at], want, tol)
+
+
 def test_run_together(gpu):
     """A routed feed-forward: token rows quantised, the experts' gated product on gathered rows, its outputs quantised, the
     down product, each step against the definition on the step's own inputs."""
@@ -377,6 +525,65 @@ def test_graph_replays(gpu, m):
         step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ys, want))
+
+
+def test_two_graphs_on_one_weight(gpu):
+    """Two graphs that share a weight and its operands, replayed in turn and on two streams at once."""
+    import torch
+    n, k, m = 512, 1536, 150
+    c = Case(gpu, 21, n, k, m)
+    ys, graphs = [out(m, n), out(m, n)], []
+    c.w.linear(c.ac, c.as_, ys[0])
+    torch.cuda.synchronize()
+    want = ys[0].clone()
+    for y in ys:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.w.linear(c.ac, c.as_, y)
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for y in ys:
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in ys)
+
+
+def test_threads(gpu):
+    """Calls of several threads at once, each on a stream of its own."""
+    import threading
+
+    import torch
+    n, k = 320, 1024
+    c = Case(gpu, 33, n, k, 40)
+    offsets = dev(np.array([0, 40], np.int32))
+    bad = []
+
+    def work():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for i in range(20):
+                y = out(40, n)
+                if i % 2:
+                    c.w.linear(c.ac, c.as_, y)
+                else:
+                    c.w.linear_grouped(c.ac, c.as_, offsets, y)
+                st.synchronize()
+                if not (np.abs(host(y) - want) <= tol).all():
+                    bad.append(i)
+
+    want, tol = mx4_ref.product(c.av, c.wv[0])
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_streams(gpu):

@@ -123,7 +123,7 @@ def test_products_refuse(fake):  # noqa: F811
         assert f(glu=1, ldy=32) == 0 and f(glu=1, ldy=31) == ARG
         for bad in (dict(w=None), dict(M=-1), dict(ldy=63), dict(y=None)):
             assert f(**bad) == ARG, (f, bad)
-        assert f(w=odd, glu=1) == LIMIT
+        assert f(w=odd, glu=1) == LIMIT and f(M=(1 << 30) + 1) == LIMIT
         fake.fake_device(1)
         assert f() == ARG      # a weight of another device
         fake.fake_device(0)
@@ -166,14 +166,32 @@ def test_products_allocate_nothing(fake):  # noqa: F811
     """)
 
 
-@pytest.mark.parametrize("experts,M", [(1, 1), (3, 5), (64, 9), (100, 4000), (300, 70)])
-def test_grouped_grid_covers_the_worst_split(fake, experts, M):  # noqa: F811
-    """However the rows are spread over the experts, the launch has a workgroup for every group of token rows."""
+GRID = [  # experts, rows, cols, gated, token rows, workgroups, threads: the form that a product takes
+    (0, 13824, 2560, 0, 1, 432, 512), (0, 151936, 1024, 0, 16, 1187, 512), (0, 2560, 6912, 0, 24, 160, 512),
+    (0, 4864, 896, 0, 48, 456, 512), (0, 2560, 2560, 0, 100, 80, 256), (0, 8192, 8192, 0, 128, 256, 256),
+    (0, 4096, 4096, 0, 1024, 512, 256), (0, 13824, 2560, 1, 512, 432, 256), (0, 8192, 8192, 0, 4096, 1024, 256),
+    (64, 2816, 2048, 1, 16384, (128 + 63) * 11 + 3, 256), (32, 2816, 2560, 1, 32, (2 + 31) * 11, 512),
+    (32, 2816, 2560, 1, 800, (13 + 31) * 22, 256),
+    # the shapes of the GPU tests of large products
+    (0, 4130, 1024, 0, 3070, 17 * 24, 256), (0, 9920, 1024, 0, 600, 78 * 5 + 2, 256), (0, 2880, 1024, 0, 1101, 23 * 18 + 2, 256),
+    (0, 1100, 2304, 0, 300, 9 * 10 + 6, 256), (7, 2304, 1536, 0, 6000, (47 + 6) * 9 + 3, 256),
+    (20, 1536, 1536, 0, 3000, (24 + 19) * 12 + 4, 256), (40, 640, 1536, 0, 4000, (63 + 39) * 5 + 2, 256),
+]
+
+
+@pytest.mark.parametrize("experts,rows,cols,glu,M,blocks,threads", GRID)
+def test_forms(fake, experts, rows, cols, glu, M, blocks, threads):  # noqa: F811
+    """The form of a product goes by its rows, columns and token rows, and by expert its grid holds every split of the rows."""
     run(fake, WEIGHT + f"""
-    experts, M = {experts}, {M}
-    g = mx4(160, 256, experts)
-    for glu in (0, 1):
-        fake.fake_reset()
-        assert lib.eif_hip_mx4_linear_grouped(g.h, X, 128, X, 8, M, None, X, None, glu, X, 160, M, None) == 0
-        assert fake.fake_launches() == 1
+    experts, rows, cols, glu, M = {experts}, {rows}, {cols}, {glu}, {M}
+    h = vp()
+    assert lib.eif_hip_mx4_weight_create(C.byref(h), max(experts, 1), rows, cols, X, cols // 2, X, cols // 32, 1, None) == 0
+    fake.fake_reset()
+    kp = lib.eif_hip_mx4_kpad(cols)
+    if experts:
+        rc = lib.eif_hip_mx4_linear_grouped(h, X, kp // 2, X, kp // 32, M, None, X, None, glu, X, rows, M, None)
+    else:
+        rc = lib.eif_hip_mx4_linear(h, X, kp // 2, X, kp // 32, None, glu, X, rows, M, None)
+    assert rc == 0 and fake.fake_launches() == 1
+    assert (fake.fake_launch_grid(0), fake.fake_launch_block(0)) == ({blocks}, {threads})
     """)
