@@ -284,16 +284,23 @@ EIF_DEV void load_bias(const float *bias, int r0, int out_rows, float *b0, float
     }
 }
 
-// The lane's four outputs of a token row. WHOLE: all four exist and y takes a 16-byte store.
-template <bool GLU, bool WHOLE>
-EIF_DEV void store_outputs(float *yr, int r0, int out_rows, v4f s0, v4f s1, const float *b0, const float *b1)
+// The lane's four outputs of a token row.
+template <bool GLU>
+EIF_DEV void outputs(v4f s0, v4f s1, const float *b0, const float *b1, float *v)
 {
-    float v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         v[j] = s0[j] + b0[j];
         if (GLU) v[j] = swiglu(v[j], s1[j] + b1[j]);
     }
+}
+
+// WHOLE: all four exist and y takes a 16-byte store.
+template <bool GLU, bool WHOLE>
+EIF_DEV void store_outputs(float *yr, int r0, int out_rows, v4f s0, v4f s1, const float *b0, const float *b1)
+{
+    float v[4];
+    outputs<GLU>(s0, s1, b0, b1, v);
     if (WHOLE) {
         *reinterpret_cast<float4 *>(yr + r0) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -663,12 +670,37 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
     auto store = [&](auto whole) {
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-            if (!ok[t]) continue;
             float *yr = a.y + (int64_t)(lo + 16 * t + n) * a.ldy;
+            if constexpr (decltype(whole)::value && OT % 2 == 0) {
+                // Two row tiles of a token row are a cache line, but in one lane. Lanes of two token rows exchange a tile
+                // each, so that a store covers the lines of eight token rows and not the halves of sixteen; whole lines can
+                // go past L2, whose room is the operands' (us, plain stores of halves / of lines / lines past L2: 4096 rows
+                // through 8192x8192 150 / 148 / 134, 16384 by expert through 2048x1408 83.7 / 78.6 / 73.8).
+                const int odd = n & 1;
+                const bool other = __shfl_xor((int)ok[t], 1, 64);
+                float *y0 = yr - odd * a.ldy + (tile0 + odd) * 16 + slot * 4, *y1 = y0 + a.ldy;
+                const bool ok0 = odd ? other : ok[t], ok1 = odd ? ok[t] : other;
 #pragma unroll
-            for (int i = 0; i < OT; ++i)
-                store_outputs<GLU, decltype(whole)::value>(yr, (tile0 + i) * 16 + slot * 4, out_rows, acc[i][t], acc[RT - OT + i][t],
-                                                        b0[i], b1[i]);
+                for (int i = 0; i < OT; i += 2) {
+                    float u[4], v[4];
+                    outputs<GLU>(acc[i][t], acc[RT - OT + i][t], b0[i], b1[i], u);
+                    outputs<GLU>(acc[i + 1][t], acc[RT - OT + i + 1][t], b0[i + 1], b1[i + 1], v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float got = xlane<1>(odd ? u[j] : v[j]);
+                        u[j] = odd ? got : u[j];
+                        v[j] = odd ? v[j] : got;
+                    }
+                    if (ok0) __builtin_nontemporal_store((v4f{u[0], u[1], u[2], u[3]}), reinterpret_cast<v4f *>(y0 + i * 16));
+                    if (ok1) __builtin_nontemporal_store((v4f{v[0], v[1], v[2], v[3]}), reinterpret_cast<v4f *>(y1 + i * 16));
+                }
+            } else {
+                if (!ok[t]) continue;
+#pragma unroll
+                for (int i = 0; i < OT; ++i)
+                    store_outputs<GLU, decltype(whole)::value>(yr, (tile0 + i) * 16 + slot * 4, out_rows, acc[i][t],
+                                                               acc[RT - OT + i][t], b0[i], b1[i]);
+            }
         }
     };
     if (a.vec && (tile0 + OT) * 16 <= out_rows)
