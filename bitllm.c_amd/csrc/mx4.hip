@@ -204,6 +204,7 @@ struct Mx4Args {
     int64_t ldy;
     int M;
     int groups;                     // of token rows
+    uint32_t code_bytes;            // of the operand rows' codes, 0 where they are 2^32 or more
     bool vec;                       // y takes 16-byte stores
     // by expert
     int experts, rows_in;
@@ -215,15 +216,19 @@ struct Mx4Args {
     bool vecx;                      // x takes loads of four elements
 };
 
-// Two MFMAs of one span: codes c0, c1 of a row tile, their scales in bytes 2 h, 2 h + 1 of sw; operand rows' in bytes
-// 0, 1 of sx.
+// One step of span H of a pair: a row tile's codes with their scale in byte 2 H + STEP of sw, operand rows' codes with
+// theirs in byte STEP of sx.
+template <int H, int STEP>
+EIF_DEV v4f step_mfma(v4f acc, v4i w, uint32_t sw, v4i x, uint32_t sx)
+{
+    const v8i a = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, b = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 2 * H + STEP, (int)sw, STEP, (int)sx);
+}
+
 template <int H>
 EIF_DEV v4f span_mfma(v4f acc, v4i w0, v4i w1, uint32_t sw, v4i x0, v4i x1, uint32_t sx)
 {
-    const v8i a0 = {w0[0], w0[1], w0[2], w0[3], 0, 0, 0, 0}, a1 = {w1[0], w1[1], w1[2], w1[3], 0, 0, 0, 0};
-    const v8i b0 = {x0[0], x0[1], x0[2], x0[3], 0, 0, 0, 0}, b1 = {x1[0], x1[1], x1[2], x1[3], 0, 0, 0, 0};
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a0, b0, acc, 4, 4, 2 * H, (int)sw, 0, (int)sx);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a1, b1, acc, 4, 4, 2 * H + 1, (int)sw, 1, (int)sx);
+    return step_mfma<H, 1>(step_mfma<H, 0>(acc, w0, sw, x0, sx), w1, sw, x1, sx);
 }
 
 // SiLU(g) u. v_exp_f32 and v_rcp_f32 are within one unit in the last place; the rounding of -g log2(e) moves the exponential by
@@ -472,19 +477,26 @@ __global__ __launch_bounds__(512) void mx4_split_kernel(Mx4Args a)
     }
 }
 
-// 16 bytes from memory straight into LDS, lane l's behind lane l - 1's.
-EIF_DEV void load_lds16(const void *src, void *dst)
+// 16 bytes from memory straight into LDS, lane l's behind lane l - 1's: a buffer load, whose counter the compiler follows exactly
+// (a global load into LDS makes it wait for everything under way at the next use of anything). Its offsets have 32 bits.
+EIF_DEV void load_lds16(__amdgpu_buffer_rsrc_t src, uint32_t lane_offset, uint32_t offset, void *dst)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, lane_offset, offset, 0, 0);
 }
 
 // Many token rows: a workgroup of four waves takes 16 TT token rows and 4 RT row tiles, RT to a wave (gated: RT / 2 of the
 // gate's and the same of the up projection's). A wave's row tiles are its own, so their codes go from memory straight
-// into registers; the token rows are shared, so they go into LDS; both PF spans ahead.
+// into registers; the token rows are shared, so they go into LDS.
+//   PF 1: token rows straight into LDS, one span ahead, and codes by steps of 128 columns, three ahead. PF 3: both three spans
+// ahead, token rows through registers; for small tiles, of which a CU has few.
 //   A span of a token tile is 16 rows of 128 bytes, 8 pieces h of 16 (piece h = 2 slot + step). A load covers eight rows,
 // whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ (n / 2)) of its half of the tile, so that the 16
 // lanes of a slot, which read one piece of 16 rows, meet 16 different groups of banks.
+//   What bounds it: 4096 rows through 8192x8192 take 128.5 us, 4.3 PFLOP/s; the matrix instructions alone run at 7.1 here (at
+// 1.7 GHz, where power holds them), and the 134 MB of outputs take 28 us of it. A span of the two workgroups on a CU is 2048
+// cycles of matrix instructions, and L2 has to bring 96 KB meanwhile. (Before whole-line loads of token rows and scales by
+// pairs of spans its request rate was the bound: 271 us. Tiles of 256x256 rows with eight waves took 5 % longer, a workgroup
+// that goes on to the next row block too: nothing covers its waits.)
 template <int RT, int TT, int PF, bool GLU, bool GROUPED>
 __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx4Args a)
 {
@@ -515,30 +527,57 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
         v4i c[RT][2];
         uint32_t s[RT];
     };
-    Weights w[R];
+    Weights w[PF > 1 ? R : 1];
+    v4i ring[PF > 1 ? 1 : 4][RT];        // PF 1: by steps, half a span each
+    uint32_t sw[PF > 1 ? 1 : 2][RT];     // pairs of spans in turn
     // Row tiles behind the matrix's last (of the last row block) are read too, the allocation holds enough of them, and not
     // stored. The same for all lanes:
-    const uint32_t tile_c = a.spans * 2048u, tile_s = (a.spans + 1) / 2 * 64u;
+    const uint32_t tile_c = a.spans * 2048u, tile_s = (a.spans + 1) / 2 * 256u;
     const uint8_t *wc[NT];
-    const uint32_t *ws[NT];
+    const uint8_t *ws[NT];
+    // A lane's offset as 32 bits that the compiler does not widen ahead of the loop: the loads take it beside a scalar address,
+    // without a 64-bit address register each.
+    auto offset = [&](uint32_t bytes) {
+        asm volatile("" : "+v"(bytes));
+        return bytes;
+    };
 #pragma unroll
     for (int h = 0; h < NT; ++h) {
         const size_t t = (size_t)expert * a.tiles + h * otiles + (rb * 4 + wave) * OT;
         wc[h] = a.wc + t * tile_c;
-        ws[h] = a.ws + t * tile_s;
+        ws[h] = reinterpret_cast<const uint8_t *>(a.ws) + t * tile_s;
     }
     auto load_weights = [&](int p, Weights &f) {
+        const uint32_t lane16 = offset(lane * 16u), lane4 = offset(lane * 4u);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const uint8_t *src = wc[i / OT] + (i % OT * tile_c + p * 2048u);
-            f.c[i][0] = *reinterpret_cast<const v4i *>(src + lane * 16);
-            f.c[i][1] = *reinterpret_cast<const v4i *>(src + 1024 + lane * 16);
+            f.c[i][0] = *reinterpret_cast<const v4i *>(src + lane16);
+            f.c[i][1] = *reinterpret_cast<const v4i *>(src + 1024 + lane16);
         }
 #pragma unroll
-        for (int i = 0; i < RT; ++i) f.s[i] = (ws[i / OT] + (i % OT * tile_s + p / 2 * 64u))[lane];
+        for (int i = 0; i < RT; ++i) f.s[i] = *reinterpret_cast<const uint32_t *>(ws[i / OT] + (i % OT * tile_s + p / 2 * 256u) + lane4);
     };
+    auto load_step = [&](int p, int step, v4i *c) {
+        const uint32_t lane16 = offset(lane * 16u);
 #pragma unroll
-    for (int k = 0; k < PF; ++k) load_weights(min(k, last), w[k]);
+        for (int i = 0; i < RT; ++i)
+            c[i] = *reinterpret_cast<const v4i *>(wc[i / OT] + (i % OT * tile_c + p * 2048u + step * 1024u) + lane16);
+    };
+    auto load_pair = [&](int q, uint32_t *v) {
+        const uint32_t lane4 = offset(lane * 4u);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) v[i] = *reinterpret_cast<const uint32_t *>(ws[i / OT] + (i % OT * tile_s + q * 256u) + lane4);
+    };
+    if constexpr (PF == 1) {
+        load_pair(0, sw[0]);
+        load_step(0, 0, ring[0]);
+        load_step(0, 1, ring[1]);
+        load_step(min(1, last), 0, ring[2]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < PF; ++k) load_weights(min(k, last), w[k]);
+    }
 
     auto operand_row = [&](int m) {
         if (m >= hi) return 0;   // row 0 is there to be read; its sums are not stored
@@ -548,23 +587,29 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
     };
     // where there are fewer half tiles than waves, or rows than threads, some stage the same
     const int half0 = PT * wave % (2 * TT);
-    const uint8_t *xr[PT];
+    const uint8_t *xr[PF == 1 ? 1 : PT];
+    uint32_t xo[PF == 1 ? PT : 1];
 #pragma unroll
     for (int j = 0; j < PT; ++j) {
         const int half = half0 + j, r = 8 * (half & 1) + (lane >> 3);
-        xr[j] = a.codes + operand_row(lo + 16 * (half >> 1) + r) * a.ldc + ((lane & 7) ^ (r >> 1)) * 16;
+        const int64_t at = operand_row(lo + 16 * (half >> 1) + r) * a.ldc + ((lane & 7) ^ (r >> 1)) * 16;
+        if constexpr (PF == 1)
+            xo[j] = (uint32_t)at;   // launch_product sees to it that it fits
+        else
+            xr[j] = a.codes + at;
     }
+    const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.codes), 0, a.code_bytes, 0x00027000);
     const uint8_t *sr[PS];
 #pragma unroll
     for (int j = 0; j < PS; ++j) sr[j] = a.scales + operand_row(lo + (j * 256 + (int)threadIdx.x) % (2 * TM) / 2) * a.lds;
     const int odd_thread = threadIdx.x & 1;
-    // one span ahead: from memory straight into LDS; more: through registers, whose loads the compiler waits for one by one
+    // PF 1: from memory straight into LDS; 3: through registers, whose loads the compiler waits for one by one
     v4i xv[R][PT];
     auto load_rows = [&](int p, v4i *v, v4i *dst) {
 #pragma unroll
         for (int j = 0; j < PT; ++j) {
             if constexpr (PF == 1)
-                load_lds16(xr[j] + (size_t)p * 128, dst + (half0 + j) * 64);
+                load_lds16(codes, xo[j], p * 128u, dst + (half0 + j) * 64);
             else
                 v[j] = *reinterpret_cast<const v4i *>(xr[j] + (size_t)p * 128);
         }
@@ -584,18 +629,18 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
 #pragma unroll
         for (int j = 0; j < PS; ++j) *reinterpret_cast<uint2 *>(&dst[(j * 256 + threadIdx.x) % (2 * TM) * 4]) = v[j];
     };
-    auto arrived = [&] {   // what the waves put into LDS is there
-        if constexpr (PF == 1) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-            __syncthreads();
-        } else {
-            // Without __syncthreads()'s wait for the loads under way. Matrix instructions may move past, memory's may not.
-            asm volatile("" ::: "memory");
+    // What the waves put into LDS is there. PF 1: this wave's loads into it too, the N loads behind them may be under way.
+    // (__syncthreads() would wait for all loads.) Matrix instructions may move past, memory's may not.
+    auto arrived = [&](auto newer) {
+        constexpr int N = decltype(newer)::value;
+        asm volatile("" ::: "memory");
+        if constexpr (PF == 1)
+            __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));   // vmcnt(N) lgkmcnt(0)
+        else
             __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0x8);
-        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0x8);
     };
     v4i *const xt[2] = {xt0, xt1};
     uint16_t *const xs[2] = {xs0, xs1};
@@ -610,34 +655,69 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
     // The span p = K modulo 4. What goes out here is for the span p + PF (near the end: the last one, again. Without a
     // branch, so that the compiler knows how many loads are under way and waits for the older ones alone).
     auto span = [&](auto k, int p) {
-        constexpr int K = decltype(k)::value, H = K & 1, Q = K >> 1, B = K % R, N = (K + PF) % R;
+        constexpr int K = decltype(k)::value, H = K & 1, Q = K >> 1;
         if (H == 0) load_scales(min(p / 2 + SV, last / 2), sv[Q % SV]);
-        load_rows(min(p + PF, last), xv[N], xt[N & 1]);
-        load_weights(min(p + PF, last), w[N]);
-        __builtin_amdgcn_sched_barrier(0);   // where the loads stand is where they go out
-        v4i b[2][2];
-        uint32_t sx[2];
-        auto read = [&](int t) {
-            b[t & 1][0] = xt[H][t * 128 + at0];
-            b[t & 1][1] = xt[H][t * 128 + at1];
-            sx[t & 1] = xs[Q][(n * 2 + H) * 4 + slot + t * 128];
-        };
-        read(0);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            if (t + 1 < TT) read(t + 1);
+        if constexpr (PF == 1) {
+            if (H == 0) load_pair(min(p / 2 + 1, last / 2), sw[Q ^ 1]);
+            load_rows(min(p + 1, last), nullptr, xt[H ^ 1]);
+            // where the loads stand is where they go out: behind these, and ahead of arrived(), the codes of two steps
             __builtin_amdgcn_sched_barrier(0);
+            constexpr int L = 2;   // pieces read ahead
+            v4i b[L + 1];
+            uint32_t sx[TT];
+            auto read = [&](int u) {   // u = step TT + t
+                const int t = u % TT;
+                b[u % (L + 1)] = xt[H][t * 128 + (u < TT ? at0 : at1)];
+                if (u < TT) sx[t] = xs[Q][(n * 2 + H) * 4 + slot + t * 128];
+            };
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
-                acc[i][t] = span_mfma<H>(acc[i][t], w[B].c[i][0], w[B].c[i][1], w[B].s[i], b[t & 1][0], b[t & 1][1], sx[t & 1]);
+            for (int u = 0; u < 2 * TT; ++u) {
+                if (u == 0) load_step(min(p + 1, last), 1, ring[(2 * H + 3) % 4]);
+                if (u == TT) load_step(min(p + 2, last), 0, ring[2 * H]);
+                if (u == 0) {
+#pragma unroll
+                    for (int l = 0; l < L; ++l) read(l);
+                }
+                if (u + L < 2 * TT) read(u + L);
+                __builtin_amdgcn_sched_barrier(0);
+                const int t = u % TT;
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    if (u < TT)
+                        acc[i][t] = step_mfma<H, 0>(acc[i][t], ring[2 * H][i], sw[Q][i], b[u % (L + 1)], sx[t]);
+                    else
+                        acc[i][t] = step_mfma<H, 1>(acc[i][t], ring[2 * H + 1][i], sw[Q][i], b[u % (L + 1)], sx[t]);
+                }
+            }
+        } else {
+            constexpr int B = K % R, N = (K + PF) % R;
+            load_rows(min(p + PF, last), xv[N], xt[N & 1]);
+            load_weights(min(p + PF, last), w[N]);
+            __builtin_amdgcn_sched_barrier(0);   // where the loads stand is where they go out
+            v4i b[2][2];
+            uint32_t sx[2];
+            auto read = [&](int t) {
+                b[t & 1][0] = xt[H][t * 128 + at0];
+                b[t & 1][1] = xt[H][t * 128 + at1];
+                sx[t & 1] = xs[Q][(n * 2 + H) * 4 + slot + t * 128];
+            };
+            read(0);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                if (t + 1 < TT) read(t + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i][t] = span_mfma<H>(acc[i][t], w[B].c[i][0], w[B].c[i][1], w[B].s[i], b[t & 1][0], b[t & 1][1], sx[t & 1]);
+            }
+            store_rows(xv[(K + 1) % R], xt[H ^ 1]);
         }
-        store_rows(xv[(K + 1) % R], xt[H ^ 1]);
         if (H == 1) store_scales(sv[(Q + 1) % SV], xs[Q ^ 1]);
-        arrived();
+        arrived(std::integral_constant<int, 2 * RT>{});
     };
     store_rows(xv[0], xt0);
     store_scales(sv[0], xs0);
-    arrived();
+    arrived(std::integral_constant<int, 0>{});
     auto pair = [&](auto q, int p) {
         constexpr int Q = decltype(q)::value;
         span(std::integral_constant<int, 2 * Q>{}, p);
@@ -756,6 +836,14 @@ int check_operand(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc
     return EIF_HIP_OK;
 }
 
+// Bytes that `rows` operand rows' codes span, 0 for 2^32 and more.
+uint32_t code_bytes(const eif_hip_mx4_weight *w, int64_t ldc, int rows)
+{
+    const int64_t row = w->spans * 128;
+    if (ldc > UINT32_MAX || (rows - 1) * ldc + row > UINT32_MAX) return 0;
+    return (uint32_t)((rows - 1) * ldc + row);
+}
+
 Mx4Args weight_args(const eif_hip_mx4_weight *w, const float *bias, float *y, int64_t ldy, int M)
 {
     Mx4Args a{};
@@ -862,6 +950,7 @@ int launch_product(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
     const int m = grouped ? (a.M - 1) / a.experts + 1 : a.M;   // token rows of a matrix
     const int64_t enough = 384;
     if (m <= 16) return launch_split<void, 1>(a, glu, grouped, st);
+    if (a.code_bytes == 0) return launch_gemm<2, 2, 3>(a, glu, grouped, st);   // the other tiles' loads have 32-bit offsets
     const int64_t g128 = groups_of(a, grouped, 128).likely, g64 = groups_of(a, grouped, 64).likely;
     if (m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= enough) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
     if (m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= enough) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
@@ -979,6 +1068,7 @@ int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_
     if ((rc = check_operand(w, codes, ldc, scales, lds)) != 0) return rc;
     Mx4Args a = weight_args(w, bias, y, ldy, M);
     a.codes = codes, a.ldc = ldc, a.scales = scales, a.lds = lds;
+    a.code_bytes = code_bytes(w, ldc, M);
     return launch_product(a, glu, false, (hipStream_t)stream);
 }
 
@@ -1012,6 +1102,7 @@ int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes
     Mx4Args a = weight_args(w, bias, y, ldy, M);
     a.codes = codes, a.ldc = ldc, a.scales = scales, a.lds = lds;
     a.rows_in = rows_in, a.index = row_index, a.offsets = offsets;
+    a.code_bytes = code_bytes(w, ldc, rows_in);
     return launch_product(a, glu, true, (hipStream_t)stream);
 }
 
