@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx
 
 // One thread a 16-byte piece of the layout: its lane's row, block and step.
 __global__ __launch_bounds__(256) void mx4_repack_kernel(const uint8_t *src, int64_t ldc, int rows, int cols, int tiles,
-                                                         int spans, uint8_t *dst, size_t pieces)
+                                                         int spans, uint8_t *dst, size_t pieces, bool vec)
 {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
@@ -161,6 +161,10 @@ __global__ __launch_bounds__(256) void mx4_repack_kernel(const uint8_t *src, int
     uint32_t w[4] = {0, 0, 0, 0};
     if (row < rows) {
         const uint8_t *s = src + (int64_t)(e * rows + row) * ldc;
+        if (vec && c0 + 32 <= cols) {   // rows aligned to 16 bytes
+            reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<const uint4 *>(s + (c0 >> 1));
+            return;
+        }
         for (int j = 0; j < 16; ++j) {
             const int c = c0 + 2 * j;
             uint32_t v = c < cols ? s[c >> 1] : 0;
@@ -1006,12 +1010,13 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     const size_t src_c = (all - 1) * ldc + ((size_t)cols + 1) / 2, src_s = (all - 1) * lds + ((size_t)cols + 31) / 32;
     uint8_t *up = nullptr;
     int rc = EIF_HIP_OK;
-    if (hipMalloc(&q.codes, cbytes + kTilesBehind * tile_codes(q.spans)) != hipSuccess ||
-        hipMalloc(&q.scales, (sdwords + kTilesBehind * tile_scales(q.spans)) * 4) != hipSuccess ||
-        (!src_on_device && hipMalloc(&up, src_c + src_s) != hipSuccess)) {
+    const size_t codes_all = cbytes + kTilesBehind * tile_codes(q.spans);
+    q.bytes = codes_all + (sdwords + kTilesBehind * tile_scales(q.spans)) * 4;
+    if (hipMalloc(&q.codes, q.bytes) != hipSuccess || (!src_on_device && hipMalloc(&up, src_c + src_s) != hipSuccess)) {
         (void)hipGetLastError();
         rc = EIF_HIP_E_NOMEM;
     }
+    if (rc == EIF_HIP_OK) q.scales = reinterpret_cast<uint32_t *>(q.codes + codes_all);   // one allocation
     if (rc == EIF_HIP_OK && !src_on_device) {
         if (hipMemcpyAsync(up, codes, src_c, hipMemcpyHostToDevice, st) != hipSuccess ||
             hipMemcpyAsync(up + src_c, scales, src_s, hipMemcpyHostToDevice, st) != hipSuccess)
@@ -1019,7 +1024,8 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
         codes = up, scales = up + src_c;
     }
     if (rc == EIF_HIP_OK) {
-        mx4_repack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, st>>>(codes, ldc, rows, cols, q.tiles, q.spans, q.codes, pieces);
+        mx4_repack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, st>>>(codes, ldc, rows, cols, q.tiles, q.spans, q.codes, pieces,
+                                                                          aligned(codes, 16) && ldc % 16 == 0);
         if (hipGetLastError() != hipSuccess) rc = EIF_HIP_E_DEVICE;
     }
     if (rc == EIF_HIP_OK) {
@@ -1028,11 +1034,9 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     }
     if (rc != EIF_HIP_E_NOMEM && hipStreamSynchronize(st) != hipSuccess && rc == EIF_HIP_OK) rc = EIF_HIP_E_DEVICE;
     if (up) (void)hipFree(up);
-    q.bytes = cbytes + sdwords * 4 + kTilesBehind * (tile_codes(q.spans) + tile_scales(q.spans) * 4);
     eif_hip_mx4_weight *h = rc == EIF_HIP_OK ? new (std::nothrow) eif_hip_mx4_weight(q) : nullptr;
     if (!h) {
         if (q.codes) (void)hipFree(q.codes);
-        if (q.scales) (void)hipFree(q.scales);
         return rc == EIF_HIP_OK ? EIF_HIP_E_NOMEM : rc;
     }
     *out = h;
@@ -1043,7 +1047,6 @@ void eif_hip_mx4_weight_destroy(eif_hip_mx4_weight *w)
 {
     if (!w) return;
     (void)hipFree(w->codes);
-    (void)hipFree(w->scales);
     delete w;
 }
 
