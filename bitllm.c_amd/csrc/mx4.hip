@@ -481,6 +481,10 @@ __global__ __launch_bounds__(512) void mx4_split_kernel(Mx4Args a)
     }
 }
 
+// Of 16 rows, two by two, the numbers 0 to 7 such that rows 0-3 and 12-15 have 0 to 3, rows 4-11 the others, and within
+// each four a number's neighbour by exclusive-or 2.
+__host__ __device__ constexpr int place(int row) { return (row & 6) ^ (row & 8 ? 5 : 0); }
+
 // 16 bytes from memory straight into LDS, lane l's behind lane l - 1's: a buffer load, whose counter the compiler follows exactly
 // (a global load into LDS makes it wait for everything under way at the next use of anything). Its offsets have 32 bits.
 EIF_DEV void load_lds16(__amdgpu_buffer_rsrc_t src, uint32_t lane_offset, uint32_t offset, void *dst)
@@ -494,8 +498,9 @@ EIF_DEV void load_lds16(__amdgpu_buffer_rsrc_t src, uint32_t lane_offset, uint32
 //   PF 1: token rows straight into LDS, one span ahead, and codes by steps of 128 columns, three ahead. PF 3: both three spans
 // ahead, token rows through registers; for small tiles, of which a CU has few.
 //   A span of a token tile is 16 rows of 128 bytes, 8 pieces h of 16 (piece h = 2 slot + step). A load covers eight rows,
-// whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ (n / 2)) of its half of the tile, so that the 16
-// lanes of a slot, which read one piece of 16 rows, meet 16 different groups of banks.
+// whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ place(n)) of its half of the tile. LDS takes a read of
+// 16 bytes a lane 16 lanes at a time, rows 0-3 and 12-15 of one slot with rows 4-11 of the next; place() gives them 16
+// different groups of banks (with n / 2 in its place they met in pairs).
 //   What bounds it: 4096 rows through 8192x8192 take 128.5 us, 4.3 PFLOP/s; the matrix instructions alone run at 7.1 here (at
 // 1.7 GHz, where power holds them), and the 134 MB of outputs take 28 us of it. A span of the two workgroups on a CU is 2048
 // cycles of matrix instructions, and L2 has to bring 96 KB meanwhile. (Before whole-line loads of token rows and scales by
@@ -596,7 +601,7 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
 #pragma unroll
     for (int j = 0; j < PT; ++j) {
         const int half = half0 + j, r = 8 * (half & 1) + (lane >> 3);
-        const int64_t at = operand_row(lo + 16 * (half >> 1) + r) * a.ldc + ((lane & 7) ^ (r >> 1)) * 16;
+        const int64_t at = operand_row(lo + 16 * (half >> 1) + r) * a.ldc + ((lane & 7) ^ place(r)) * 16;
         if constexpr (PF == 1)
             xo[j] = (uint32_t)at;   // launch_product sees to it that it fits
         else
@@ -655,7 +660,7 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
 
     v4f acc[RT][TT] = {};
     // where a piece lies that this lane reads: row n's 2 slot and 2 slot + 1
-    const int at0 = 64 * (n >> 3) + 8 * (n & 7) + ((2 * slot) ^ (n >> 1)), at1 = at0 ^ 1;
+    const int at0 = 64 * (n >> 3) + 8 * (n & 7) + ((2 * slot) ^ place(n)), at1 = at0 ^ 1;
     // The span p = K modulo 4. What goes out here is for the span p + PF (near the end: the last one, again. Without a
     // branch, so that the compiler knows how many loads are under way and waits for the older ones alone).
     auto span = [&](auto k, int p) {
@@ -942,25 +947,27 @@ int launch_gemm(Mx4Args a, bool glu, bool grouped, hipStream_t st)
     return EIF_HIP_OK;
 }
 
-// The form of a product of quantised rows: the largest tile that still gives the CUs (256) workgroups enough, 1.5 each or
-// more; of a few rows the split form. By expert a tile of more token rows than an expert has on average is mostly empty.
-// Measured (us; 256 rows x 128 tokens / 128x128 / 128x64 / 128x32 three spans ahead / split):
-//   4096 rows, 8192x8192 151 / 173 / 218 / 325 / -; 512, gated 13824x2560 17.8 / 16.7 / 18.9 / 24.4 / 55
-//   1024, 4096x4096 24.4 / 17.4 / 16.4 / 22.4 / -; 256, 2560x6912 34 / 23.4 / 19.1 / 12.2 / 25; 128, 8192x8192 38 / 26 / 21 /
-//   13.9 / 50; 100, 2560x2560 14.8 / 9.9 / 7.1 / 6.5 / 8.0; 48, 4864x896 - / 5.5 / 4.5 / 4.3 / 3.6; 24, 2560x6912 - / 18.6 /
-//   16.8 / 16 / 6.1; by expert, gated 2816 rows: 16384 rows to 64 103 / 112 / 119 / 160 / -, 800 to 32 35 / 37 / 31 / 35 / 42.
+// The form of a product of quantised rows: the largest tile that still gives the 256 CUs workgroups enough (200; 256; 160); of a few
+// rows the split form. By expert a tile of more token rows than an expert has on average is mostly empty. Measured (us; 256
+// rows x 128 tokens / 128x128 / 128x64 / 128x32 three spans ahead / split; in brackets the workgroups of the first three):
+//   4096 rows, 8192x8192 133 / 149 / 187 / 291 / 1615 (1024, 2048, 4096); 512, gated 13824x2560 15.0 / 16.2 / 18.5 / 25.1 / 87 (216,
+//   432, 864); 800, 5120x5120 20.8 / 23.4 / 23.3 / 26.1 / - (140, 280, 520); 1024, 4096x4096 17.6 / 14.2 / 14.9 / 21.6 / 103 (128,
+//   256, 512); 1500, 2560x2560 13.3 / 10.3 / 10.3 / 15.7 / - (120, 240, 480); 384, 8192x8192 29 / 21 / 22 / 29 / - (96, 192,
+//   384); 640, 2560x6912 26 / 18.3 / 15.2 / 18.0 / - (50, 100, 200); 128, 8192x8192 29 / 20 / 16.9 / 13.8 / 53 (32, 64, 128); 256,
+//   2560x6912 26 / 18.1 / 14.8 / 12.1 / 37 (20, 40, 80); 100, 2560x2560 12.1 / 8.1 / 6.0 / 6.3 / 10.3; 32, 8192x8192 28 / 19 / 16 /
+//   13.5 / 15.5; 600, 1024x1024 - / - / 4.3 / 4.2 / 8.2; 60, 4096x1024 - / - / 4.1 / 3.9 / 3.6; 48, 4864x896 7.4 / 5.2 / 4.0 / 4.0 / 3.6; 24, 2560x6912 24 / 16 / 14 / 11.6 / 6.1; by expert, gated 2816 rows: 16384
+//   rows to 64 99 / 113 / 121 / 163 / 389, 800 to 32 37 / 36 / 30 / 36 / 38; 2048 to 32 of 2048x1408 18.7 / 18.0 / 15.3 / 18.6 / 54.
 int launch_product(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
     const int m = grouped ? (a.M - 1) / a.experts + 1 : a.M;   // token rows of a matrix
-    const int64_t enough = 384;
     if (m <= 16) return launch_split<void, 1>(a, glu, grouped, st);
     if (a.code_bytes == 0) return launch_gemm<2, 2, 3>(a, glu, grouped, st);   // the other tiles' loads have 32-bit offsets
     const int64_t g128 = groups_of(a, grouped, 128).likely, g64 = groups_of(a, grouped, 64).likely;
-    if (m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= enough) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
-    if (m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= enough) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
-    if (gemm_blocks<2, 4>(a, glu, g64) >= enough) return launch_gemm<2, 4, 1>(a, glu, grouped, st);
-    if (a.spans >= 8 && gemm_blocks<2, 2>(a, glu, groups_of(a, grouped, 32).likely) >= 64)
-        return launch_gemm<2, 2, 3>(a, glu, grouped, st);
+    if (m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= 200) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
+    if (m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= 256) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
+    if (gemm_blocks<2, 4>(a, glu, g64) >= 160) return launch_gemm<2, 4, 1>(a, glu, grouped, st);
+    const int64_t small = gemm_blocks<2, 2>(a, glu, groups_of(a, grouped, 32).likely);
+    if (small >= 64 && small * a.spans >= 400) return launch_gemm<2, 2, 3>(a, glu, grouped, st);
     return m <= 32 ? launch_split<void, 2>(a, glu, grouped, st) : launch_split<void, 1>(a, glu, grouped, st);
 }
 

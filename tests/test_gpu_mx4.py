@@ -368,8 +368,8 @@ def test_linear_large(gpu, n, m, k, glu):
         check_on_gpu(y, want, tol)
 
 
-@pytest.mark.parametrize("n,m,experts", [(2304, 6000, 7), (1536, 3000, 20), (640, 4000, 40), (1100, 700, 9)])
-@pytest.mark.parametrize("k", [300, 1536])
+@pytest.mark.parametrize("n,m,experts", [(2304, 6000, 7), (1280, 3000, 20), (640, 3600, 40), (1100, 700, 9)])
+@pytest.mark.parametrize("k", [300, 1536, 2304])
 @pytest.mark.parametrize("glu", [False, True])
 def test_grouped_large(gpu, n, m, experts, k, glu):
     import torch

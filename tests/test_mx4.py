@@ -168,14 +168,16 @@ def test_products_allocate_nothing(fake):  # noqa: F811
 
 GRID = [  # experts, rows, cols, gated, token rows, workgroups, threads: the form that a product takes
     (0, 13824, 2560, 0, 1, 432, 512), (0, 151936, 1024, 0, 16, 1187, 512), (0, 2560, 6912, 0, 24, 160, 512),
-    (0, 4864, 896, 0, 48, 456, 512), (0, 2560, 2560, 0, 100, 80, 256), (0, 8192, 8192, 0, 128, 256, 256),
-    (0, 4096, 4096, 0, 1024, 512, 256), (0, 13824, 2560, 1, 512, 432, 256), (0, 8192, 8192, 0, 4096, 1024, 256),
+    (0, 4864, 896, 0, 48, 456, 512), (0, 2560, 2560, 0, 100, 80, 256), (0, 1024, 1024, 0, 600, 152, 256), (0, 8192, 8192, 0, 128, 256, 256),
+    (0, 4096, 4096, 0, 1024, 256, 256), (0, 13824, 2560, 1, 512, 216, 256),
+    (0, 4096, 4096, 0, 512, 256, 256), (0, 8192, 8192, 0, 4096, 1024, 256),
     (64, 2816, 2048, 1, 16384, (128 + 63) * 11 + 3, 256), (32, 2816, 2560, 1, 32, (2 + 31) * 11, 512),
     (32, 2816, 2560, 1, 800, (13 + 31) * 22, 256),
     # the shapes of the GPU tests of large products
     (0, 4130, 1024, 0, 3070, 17 * 24, 256), (0, 9920, 1024, 0, 600, 78 * 5 + 2, 256), (0, 2880, 1024, 0, 1101, 23 * 18 + 2, 256),
     (0, 1100, 2304, 0, 300, 9 * 10 + 6, 256), (7, 2304, 1536, 0, 6000, (47 + 6) * 9 + 3, 256),
-    (20, 1536, 1536, 0, 3000, (24 + 19) * 12 + 4, 256), (40, 640, 1536, 0, 4000, (63 + 39) * 5 + 2, 256),
+    (20, 1280, 1536, 0, 3000, (24 + 19) * 10 + 2, 256), (40, 640, 1536, 0, 3600, (57 + 39) * 5, 256),
+    (9, 1100, 2304, 0, 700, (22 + 8) * 9 + 2, 256),
 ]
 
 
