@@ -38,7 +38,8 @@ int eif_hip_mx4_kpad(int cols);
  *   codes [rows, ldc] (16-byte aligned, ldc a multiple of 16, >= kpad / 2) and scales [rows, lds] (8-byte aligned, lds a
  *   multiple of 8, >= kpad / 32): columns cols .. kpad - 1 get zero codes, blocks without columns scale 0. Bytes beyond are
  *   left as they were. Both may be NULL;
- *   values [rows, ldv] FP32 or NULL: what the codes stand for.                                                */
+ *   values [rows, ldv] FP32 or NULL: what the codes stand for.
+ * cols beyond 2^24, or more rows than a launch holds (2^33 runs of 256 columns): EIF_HIP_E_LIMIT. */
 int eif_hip_mx4_quant_rows(const void *x, int type, int64_t ldx, int rows, int cols, uint8_t *codes, int64_t ldc,
                            uint8_t *scales, int64_t lds, float *values, int64_t ldv, void *stream);
 
