@@ -802,6 +802,7 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
 
 constexpr int kMaxCols = 1 << 24;
 constexpr int kMaxRows = 1 << 30;
+constexpr int kMaxExperts = 4096;    // a workgroup of a product by expert goes over all offsets
 constexpr int kTilesBehind = 15;   // row tiles that a product may read behind the last
 constexpr int kRowsMaxM = 8, kRowsMaxCols = 16384;
 
@@ -1002,7 +1003,7 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     *out = nullptr;
     if (!codes || !scales || experts < 1 || rows < 1 || cols < 1) return EIF_HIP_E_ARG;
     if (ldc < ((int64_t)cols + 1) / 2 || lds < ((int64_t)cols + 31) / 32) return EIF_HIP_E_ARG;
-    if (cols > kMaxCols || rows > kMaxRows) return EIF_HIP_E_LIMIT;
+    if (cols > kMaxCols || rows > kMaxRows || experts > kMaxExperts) return EIF_HIP_E_LIMIT;
     eif_hip_mx4_weight q{};
     q.experts = experts, q.rows = rows, q.cols = cols, q.tiles = eif_ceil_div(rows, 16), q.spans = spans_of(cols);
     if ((int64_t)experts * q.tiles > INT32_MAX) return EIF_HIP_E_LIMIT;

@@ -258,7 +258,7 @@ def grouped_want(c, offsets, idx, m, n, glu, bias):
 GROUPED = [  # experts, rows, cols, tokens, rows of y, spread
     (1, 64, 300, 5, 9, "ragged"), (4, 33, 100, 7, 1, "ragged"), (8, 96, 512, 8, 32, "ragged"), (32, 160, 1000, 3, 24, "ragged"),
     (3, 256, 257, 50, 200, "ragged"), (5, 128, 640, 300, 700, "ragged"), (70, 64, 256, 20, 150, "ragged"), (200, 32, 64, 40, 500, "ragged"),
-    (6, 96, 768, 200, 333, "one"), (129, 64, 300, 64, 64, "last"), (2, 640, 2560, 600, 1200, "ragged"),
+    (6, 96, 768, 200, 333, "one"), (129, 64, 300, 64, 64, "last"), (1500, 16, 64, 30, 900, "ragged"), (2, 640, 2560, 600, 1200, "ragged"),
 ]
 
 
@@ -441,6 +441,24 @@ def test_offsets_beyond_32_bits(gpu, m, n):
         y.fill_(float("nan"))
         c.w.linear_rows(x, y)
         check(y, *want)
+
+
+@pytest.mark.parametrize("m,n", [(300, 4096), (600, 10240)])
+def test_operand_rows_behind_31_bits(gpu, m, n):
+    """Operand rows that span between 2^31 and 2^32 bytes, through the forms whose loads take 32-bit offsets."""
+    import torch
+    k = 1000
+    w, wv, ac, as_, av, bias = large(gpu, n, k, m)
+    far = (7 << 29) // m // 16 * 16
+    codes = torch.empty(far * m, dtype=torch.uint8, device="cuda").as_strided((m, 512), (far, 1))
+    codes.copy_(ac)
+    y = out(m, n)
+    w.linear(codes, as_, y, bias[0])
+    check_on_gpu(y, *product_on_gpu(av, wv[0], bias[0], False))
+    idx = torch.arange(m - 1, -1, -1, device="cuda", dtype=torch.int32)
+    y = out(m, n)
+    w.linear_grouped(codes, as_, dev(np.array([0, m], np.int32)), y, idx, bias)
+    check_on_gpu(y, *product_on_gpu(av.flip(0), wv[0], bias[0], False))
 
 
 @pytest.mark.parametrize("m", [3, 60, 200])

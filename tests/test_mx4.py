@@ -79,7 +79,8 @@ def test_create_refuses_and_gives_back(fake):  # noqa: F811
                 dict(lds=1), dict(cols=65, ldc=32), dict(cols=65, ldc=33)):
         assert create(**bad) == ARG, bad
     assert create(cols=65, ldc=33, lds=3) == 0
-    assert create(rows=(1 << 30) + 1) == LIMIT and create(cols=(1 << 24) + 1, ldc=1 << 24, lds=1 << 20) == LIMIT and create(experts=1 << 20, rows=1 << 20) == LIMIT
+    assert create(rows=(1 << 30) + 1) == LIMIT and create(cols=(1 << 24) + 1, ldc=1 << 24, lds=1 << 20) == LIMIT and create(experts=4097) == LIMIT and create(experts=4096) == 0
+    assert create(experts=4096, rows=1 << 30, cols=1, ldc=1, lds=1) == LIMIT
     for dev in (0, 1):
         fake.fake_reset(); fake.fake_fail_malloc(1)
         assert create(dev=dev) == -3 and fake.fake_live() == 0
@@ -175,7 +176,7 @@ GRID = [  # experts, rows, cols, gated, token rows, workgroups, threads: the for
     (32, 2816, 2560, 1, 800, (13 + 31) * 22, 256),
     # the shapes of the GPU tests of large products
     (0, 4130, 1024, 0, 3070, 17 * 24, 256), (0, 9920, 1024, 0, 600, 78 * 5 + 2, 256), (0, 2880, 1024, 0, 1101, 23 * 18 + 2, 256),
-    (0, 1100, 2304, 0, 300, 9 * 10 + 6, 256), (7, 2304, 1536, 0, 6000, (47 + 6) * 9 + 3, 256),
+    (0, 1100, 2304, 0, 300, 9 * 10 + 6, 256), (0, 4096, 1024, 0, 300, 160, 256), (0, 10240, 1024, 0, 600, 200, 256), (7, 2304, 1536, 0, 6000, (47 + 6) * 9 + 3, 256),
     (20, 1280, 1536, 0, 3000, (24 + 19) * 10 + 2, 256), (40, 640, 1536, 0, 3600, (57 + 39) * 5, 256),
     (9, 1100, 2304, 0, 700, (22 + 8) * 9 + 2, 256),
 ]
