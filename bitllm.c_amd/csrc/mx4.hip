@@ -501,7 +501,7 @@ EIF_DEV void load_lds16(__amdgpu_buffer_rsrc_t src, uint32_t lane_offset, uint32
 // whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ place(n)) of its half of the tile. LDS takes a read of
 // 16 bytes a lane 16 lanes at a time, rows 0-3 and 12-15 of one slot with rows 4-11 of the next; place() gives them 16
 // different groups of banks (with n / 2 in its place they met in pairs).
-//   What bounds it: 4096 rows through 8192x8192 take 128.5 us, 4.3 PFLOP/s; the matrix instructions alone run at 7.1 here (at
+//   What bounds it: 4096 rows through 8192x8192 take 126 to 133 us, 4.1 to 4.4 PFLOP/s; the matrix instructions alone run at 7.1 here (at
 // 1.7 GHz, where power holds them), and the 134 MB of outputs take 28 us of it. A span of the two workgroups on a CU is 2048
 // cycles of matrix instructions, and L2 has to bring 96 KB meanwhile. (Before whole-line loads of token rows and scales by
 // pairs of spans its request rate was the bound: 271 us. Tiles of 256x256 rows with eight waves took 5 % longer, a workgroup
