@@ -145,11 +145,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx
 
 // ---- the resident layout ----
 
-// One thread a 16-byte piece of the layout: its lane's row, block and step.
+// One thread a 16-byte piece of the layout, from piece `first` on: its lane's row, block and step.
 __global__ __launch_bounds__(256) void mx4_repack_kernel(const uint8_t *src, int64_t ldc, int rows, int cols, int tiles,
-                                                         int spans, uint8_t *dst, size_t pieces, bool vec)
+                                                         int spans, uint8_t *dst, size_t first, size_t pieces, bool vec)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t i = first + (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
     const int lane = (int)(i & 63), step = (int)(i >> 6) & 1;
     size_t t = i >> 7;
@@ -175,11 +175,11 @@ __global__ __launch_bounds__(256) void mx4_repack_kernel(const uint8_t *src, int
     reinterpret_cast<uint4 *>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One thread a dword of scales: the lane's four blocks of a pair of spans.
+// One thread a dword of scales, from dword `first` on: the lane's four blocks of a pair of spans.
 __global__ __launch_bounds__(256) void mx4_repack_scales_kernel(const uint8_t *src, int64_t lds, int rows, int cols,
-                                                                int tiles, int spans, uint32_t *dst, size_t n)
+                                                                int tiles, int spans, uint32_t *dst, size_t first, size_t n)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t i = first + (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const int lane = (int)(i & 63), pairs = (spans + 1) / 2, blocks = (cols + 31) / 32;
     size_t t = i >> 6;
@@ -800,6 +800,8 @@ __global__ __launch_bounds__(256, RT * TT <= 32 ? 2 : 1) void mx4_gemm_kernel(Mx
 
 // ---- host ----
 
+constexpr int64_t kLaunchThreads = UINT32_MAX;   // threads that a launch holds at most
+constexpr int64_t kLaunchBlocks = kLaunchThreads / 256;   // workgroups of 256
 constexpr int kMaxCols = 1 << 24;
 constexpr int kMaxRows = 1 << 30;
 constexpr int kMaxExperts = 4096;    // a workgroup of a product by expert goes over all offsets
@@ -815,15 +817,21 @@ int launch_quant(const void *x, int64_t ldx, int rows, int cols, uint8_t *codes,
                  int64_t lds, float *values, int64_t ldv, hipStream_t st)
 {
     const int spans = spans_of(cols);
-    const int64_t blocks = ((int64_t)rows * spans + 3) / 4;
-    if (blocks > INT32_MAX) return EIF_HIP_E_LIMIT;
-    const bool vv = aligned(values, 16) && ldv % 4 == 0;
-    const T *xt = static_cast<const T *>(x);
-    if (aligned(x, 4 * sizeof(T)) && ldx % 4 == 0 && cols % 4 == 0)
-        quant_rows_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv, vv);
-    else
-        quant_rows_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(xt, ldx, rows, cols, spans, codes, ldc, scales, lds, values, ldv, vv);
-    EIF_HIP_LAUNCHED();
+    if (((int64_t)rows * spans + 3) / 4 > INT32_MAX) return EIF_HIP_E_LIMIT;
+    const bool vec = aligned(x, 4 * sizeof(T)) && ldx % 4 == 0 && cols % 4 == 0, vv = aligned(values, 16) && ldv % 4 == 0;
+    const int64_t per = kLaunchBlocks * 4 / spans;   // rows of a launch
+    for (int64_t row = 0; row < rows; row += per) {
+        const int n = (int)std::min(per, rows - row);
+        const unsigned blocks = (unsigned)(((int64_t)n * spans + 3) / 4);
+        const T *xt = static_cast<const T *>(x) + row * ldx;
+        uint8_t *c = codes ? codes + row * ldc : nullptr, *s = scales ? scales + row * lds : nullptr;
+        float *v = values ? values + row * ldv : nullptr;
+        if (vec)
+            quant_rows_kernel<T, true><<<blocks, 256, 0, st>>>(xt, ldx, n, cols, spans, c, ldc, s, lds, v, ldv, vv);
+        else
+            quant_rows_kernel<T, false><<<blocks, 256, 0, st>>>(xt, ldx, n, cols, spans, c, ldc, s, lds, v, ldv, vv);
+        EIF_HIP_LAUNCHED();
+    }
     return EIF_HIP_OK;
 }
 
@@ -878,7 +886,7 @@ template <typename X, int TT, int KW, int D>
 int launch_split_as(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
     const int64_t blocks = groups_of(a, grouped, 16 * TT).grid * eif_ceil_div(glu ? a.tiles / 2 : a.tiles, 8 / KW);
-    if (blocks > INT32_MAX) return EIF_HIP_E_LIMIT;
+    if (blocks > kLaunchThreads / 512) return EIF_HIP_E_LIMIT;
     const unsigned g = (unsigned)blocks;
     if constexpr (std::is_void<X>::value) {
         if (glu)
@@ -934,10 +942,10 @@ int64_t gemm_blocks(const Mx4Args &a, bool glu, int64_t groups)
 template <int RT, int TT, int PF>
 int launch_gemm(Mx4Args a, bool glu, bool grouped, hipStream_t st)
 {
-    const int64_t groups = groups_of(a, grouped, 16 * TT).grid, blocks = gemm_blocks<RT, TT>(a, glu, groups);
-    if (blocks > (1 << 28)) return EIF_HIP_E_LIMIT;
+    const int64_t groups = groups_of(a, grouped, 16 * TT).grid, blocks = (gemm_blocks<RT, TT>(a, glu, groups) + 7) / 8 * 8;
+    if (blocks > kLaunchBlocks) return EIF_HIP_E_LIMIT;
     a.groups = (int)groups;
-    const unsigned g = (unsigned)(blocks + 7) / 8 * 8;
+    const unsigned g = (unsigned)blocks;
     if (glu)
         grouped ? mx4_gemm_kernel<RT, TT, PF, true, true><<<g, 256, 0, st>>>(a)
                 : mx4_gemm_kernel<RT, TT, PF, true, false><<<g, 256, 0, st>>>(a);
@@ -1010,8 +1018,7 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     if (hipGetDevice(&q.device) != hipSuccess) return EIF_HIP_E_DEVICE;
     const size_t tiles = (size_t)experts * q.tiles;
     const size_t cbytes = tiles * tile_codes(q.spans), sdwords = tiles * tile_scales(q.spans);
-    const size_t pieces = cbytes / 16;
-    if (pieces > (size_t)INT32_MAX * 256) return EIF_HIP_E_LIMIT;
+    const size_t pieces = cbytes / 16, per = (size_t)kLaunchBlocks * 256;   // of a launch
     hipStream_t st = (hipStream_t)stream;
     // host rows go up as they lie, up to the last row's end
     const size_t all = (size_t)experts * rows;
@@ -1031,13 +1038,15 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
             rc = EIF_HIP_E_DEVICE;
         codes = up, scales = up + src_c;
     }
-    if (rc == EIF_HIP_OK) {
-        mx4_repack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, st>>>(codes, ldc, rows, cols, q.tiles, q.spans, q.codes, pieces,
-                                                                          aligned(codes, 16) && ldc % 16 == 0);
+    const bool vec = aligned(codes, 16) && ldc % 16 == 0;
+    for (size_t i = 0; i < pieces && rc == EIF_HIP_OK; i += per) {
+        const unsigned blocks = (unsigned)((std::min(per, pieces - i) + 255) / 256);
+        mx4_repack_kernel<<<blocks, 256, 0, st>>>(codes, ldc, rows, cols, q.tiles, q.spans, q.codes, i, pieces, vec);
         if (hipGetLastError() != hipSuccess) rc = EIF_HIP_E_DEVICE;
     }
-    if (rc == EIF_HIP_OK) {
-        mx4_repack_scales_kernel<<<(unsigned)((sdwords + 255) / 256), 256, 0, st>>>(scales, lds, rows, cols, q.tiles, q.spans, q.scales, sdwords);
+    for (size_t i = 0; i < sdwords && rc == EIF_HIP_OK; i += per) {
+        const unsigned blocks = (unsigned)((std::min(per, sdwords - i) + 255) / 256);
+        mx4_repack_scales_kernel<<<blocks, 256, 0, st>>>(scales, lds, rows, cols, q.tiles, q.spans, q.scales, i, sdwords);
         if (hipGetLastError() != hipSuccess) rc = EIF_HIP_E_DEVICE;
     }
     if (rc != EIF_HIP_E_NOMEM && hipStreamSynchronize(st) != hipSuccess && rc == EIF_HIP_OK) rc = EIF_HIP_E_DEVICE;

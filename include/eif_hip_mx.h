@@ -39,7 +39,8 @@ int eif_hip_mx4_kpad(int cols);
  *   multiple of 8, >= kpad / 32): columns cols .. kpad - 1 get zero codes, blocks without columns scale 0. Bytes beyond are
  *   left as they were. Both may be NULL;
  *   values [rows, ldv] FP32 or NULL: what the codes stand for.
- * cols beyond 2^24, or more rows than a launch holds (2^33 runs of 256 columns): EIF_HIP_E_LIMIT. */
+ * One launch up to 2^26 - 4 runs of 256 columns (a last one of fewer counts), several beyond. cols beyond 2^24, or
+ * 2^33 - 3 such runs and more: EIF_HIP_E_LIMIT. */
 int eif_hip_mx4_quant_rows(const void *x, int type, int64_t ldx, int rows, int cols, uint8_t *codes, int64_t ldc,
                            uint8_t *scales, int64_t lds, float *values, int64_t ldv, void *stream);
 
@@ -63,7 +64,8 @@ int eif_hip_mx4_weight_info(const eif_hip_mx4_weight *w, int *experts, int *rows
  * glu != 0: the matrix stacks gate rows (0 .. rows/2 - 1) over up rows (rows/2 .. rows - 1); y [M, rows/2] =
  * SiLU(g) u = (g / (1 + e^-g)) u of the two products with their biases, the exponential and the quotient with the GPU's own
  * instructions (beside the rounding of g, 2^-21 of the result). rows a multiple of 32, else EIF_HIP_E_LIMIT.
- * M beyond 2^30, and products of more workgroups than a launch holds (2^28): EIF_HIP_E_LIMIT.               */
+ * M beyond 2^30, and products that take 2^32 threads and more (256 for 32 to 128 token rows and 128 or 256 matrix rows;
+ * of up to 16 token rows a matrix, and of small matrices, 512 for 16 or 32 and 16 to 128): EIF_HIP_E_LIMIT. */
 int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales, int64_t lds,
                        const float *bias, int glu, float *y, int64_t ldy, int M, void *stream);
 

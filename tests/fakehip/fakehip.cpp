@@ -3,8 +3,11 @@
 // before the library, its symbols take the place of the runtime's.
 #include <hip/hip_runtime_api.h>
 
+#include <sys/mman.h>
+
 #include <cstdlib>
 #include <cstring>
+#include <map>
 
 namespace {
 
@@ -21,6 +24,8 @@ hipError_t g_last;
 dim3 g_grid, g_block;
 size_t g_shmem;
 hipStream_t g_stream;
+
+std::map<void *, size_t> g_large;   // allocations that only have addresses: nothing touches them
 
 hipError_t set(hipError_t e)
 {
@@ -49,14 +54,27 @@ void fake_capturing(int on) { g_capturing = on; }
 hipError_t hipMalloc(void **p, size_t n)
 {
     ++g_mallocs;
-    if (g_fail_malloc || !(*p = calloc(1, n))) return set(hipErrorOutOfMemory);
+    if (g_fail_malloc) return set(hipErrorOutOfMemory);
+    if (n >> 32) {
+        *p = mmap(nullptr, n, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS | MAP_NORESERVE, -1, 0);
+        if (*p == MAP_FAILED) return set(hipErrorOutOfMemory);
+        g_large[*p] = n;
+    } else if (!(*p = calloc(1, n))) {
+        return set(hipErrorOutOfMemory);
+    }
     ++g_live;
     return hipSuccess;
 }
 hipError_t hipFree(void *p)
 {
     if (p) --g_live;
-    free(p);
+    const auto l = g_large.find(p);
+    if (l == g_large.end()) {
+        free(p);
+    } else {
+        munmap(p, l->second);
+        g_large.erase(l);
+    }
     return hipSuccess;
 }
 hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind, hipStream_t)
@@ -114,6 +132,7 @@ hipError_t hipLaunchKernel(const void *fn, dim3 grid, dim3 block, void **args, s
         g_launch[i] = {fn, st, nullptr, grid, block};
         if (g_arg1) memcpy(&g_launch[i].arg1, args[1], sizeof(void *));
     }
+    if ((unsigned long long)grid.x * block.x >> 32) return set(hipErrorInvalidConfiguration);   // as the runtime does
     return set(i == g_fail_launch ? hipErrorLaunchFailure : hipSuccess);
 }
 
