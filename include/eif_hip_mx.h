@@ -63,7 +63,8 @@ int eif_hip_mx4_weight_info(const eif_hip_mx4_weight *w, int *experts, int *rows
  * partial sums leave FP32's range as an infinity or NaN.
  * glu != 0: the matrix stacks gate rows (0 .. rows/2 - 1) over up rows (rows/2 .. rows - 1); y [M, rows/2] =
  * SiLU(g) u = (g / (1 + e^-g)) u of the two products with their biases, the exponential and the quotient with the GPU's own
- * instructions (beside the rounding of g, 2^-21 of the result). rows a multiple of 32, else EIF_HIP_E_LIMIT.
+ * instructions: of the FP32 sums g and u, within (2^-21 + 2^-23 |g|) |y| + 2^-119 |u| + 2^-149 (below g = -87.3 y may be 0).
+ * rows a multiple of 32, else EIF_HIP_E_LIMIT.
  * M beyond 2^30, and products that take 2^32 threads and more (256 for 32 to 128 token rows and 128 or 256 matrix rows;
  * of up to 16 token rows a matrix, and of small matrices, 512 for 16 or 32 and 16 to 128): EIF_HIP_E_LIMIT. */
 int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales, int64_t lds,

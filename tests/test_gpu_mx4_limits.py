@@ -55,3 +55,41 @@ def test_weight_beyond_a_launch(gpu):
     y = y.view(times, period)
     assert torch.equal(y[:-1], want.expand(times - 1, period)) and torch.equal(y[-1, :tail], want[0, :tail])
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("form,n,m", [("rows", 320, 3), ("linear", 320, 12), ("linear", 640, 28), ("linear", 2208, 300), ("linear", 5760, 1101),
+                                      ("linear", 19840, 600), ("grouped", 320, 60), ("grouped", 2560, 3000)])
+def test_gates_far_below_zero(gpu, form, n, m):
+    """SiLU(g) u where e^-g nears the end of FP32's range and passes it. The sums are zeros, so that g and u are the biases alone.
+    -g log2(e) is off by two roundings, which move the exponential by |g| 2^-23; the exponential, the quotient and the products
+    come to 2^-21. From e^-g = 2^126 on the quotient may be 0, where |SiLU(g)| <= 87.4 2^-126 < 2^-119; a result below the
+    smallest normal number is off by half a step of its own."""
+    import torch
+    k, h, experts = 64, n // 2, 5 if form == "grouped" else 1
+    w = gpu.Mx4Weight(n, k, np.zeros((experts * n, k // 2), np.uint8), np.zeros((experts * n, k // 32), np.uint8), experts=experts)
+    rng = np.random.default_rng(n + m)
+    g = np.concatenate([[-0.0, 0.0, -87.25, -87.5, -88.0, -88.75, -89.0, -92.0, -104.0, -174.0, -180.0, -190.0, -300.0, -1e9, 88.0],
+                        rng.uniform(-60, -40, h // 4), rng.uniform(-200, 90, h)])[:h].astype(np.float32)
+    u = rng.choice([1.0, -1e6, 1e30, -3e38, 3e-3], h).astype(np.float32)
+    bias = dev(np.tile(np.concatenate([g, u]), (experts, 1)))
+    y = torch.full((m, h), float("nan"), device="cuda")
+    x = dev(mx4_ref.activations(rng, m, k))
+    if form == "rows":
+        w.linear_rows(x, y, bias[0], glu=True)
+    else:
+        codes = torch.zeros((m, w.kpad // 2), dtype=torch.uint8, device="cuda")
+        scales = torch.zeros((m, w.kpad // 32), dtype=torch.uint8, device="cuda")
+        gpu.mx4_quant_rows(x, codes, scales)
+        if form == "grouped":
+            w.linear_grouped(codes, scales, dev(np.linspace(0, m, experts + 1).astype(np.int32)), y, bias=bias, glu=True)
+        else:
+            w.linear(codes, scales, y, bias[0], glu=True)
+    torch.cuda.synchronize()
+    g, u = g.astype(np.float64), u.astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = g / (1.0 + np.exp(-g)) * u
+    tol = np.abs(want) * (2.0 ** -21 + np.abs(g) * 2.0 ** -23) + 2.0 ** -119 * np.abs(u) + 2.0 ** -149
+    keep = np.abs(want) < 3.4e38
+    got = y.cpu().numpy().astype(np.float64)
+    bad = (np.abs(got - want) > tol) & keep | ~keep & ~np.isinf(got)
+    assert not bad.any(), [(g[c], u[c], got[r, c], want[c]) for r, c in np.argwhere(bad)[:5]]
