@@ -973,14 +973,18 @@ int launch_product(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
     const int m = grouped ? (a.M - 1) / a.experts + 1 : a.M;   // token rows of a matrix
     if (m <= 16) return launch_split<void, 1>(a, glu, grouped, st);
-    if (a.code_bytes == 0) return launch_gemm<2, 2, 3>(a, glu, grouped, st);   // the other tiles' loads have 32-bit offsets
     const int64_t g128 = groups_of(a, grouped, 128).likely, g64 = groups_of(a, grouped, 64).likely;
-    if (m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= 200) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
-    if (m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= 256) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
-    if (gemm_blocks<2, 4>(a, glu, g64) >= 160) return launch_gemm<2, 4, 1>(a, glu, grouped, st);
+    const bool wide = m >= 96 && gemm_blocks<4, 8>(a, glu, g128) >= 200, middle = m >= 96 && gemm_blocks<2, 8>(a, glu, g128) >= 256;
+    const bool narrow = gemm_blocks<2, 4>(a, glu, g64) >= 160;
     const int64_t small = gemm_blocks<2, 2>(a, glu, groups_of(a, grouped, 32).likely);
-    if (small >= 64 && small * a.spans >= 400) return launch_gemm<2, 2, 3>(a, glu, grouped, st);
-    return m <= 32 ? launch_split<void, 2>(a, glu, grouped, st) : launch_split<void, 1>(a, glu, grouped, st);
+    if (!wide && !middle && !narrow && (small < 64 || small * a.spans < 400))
+        return m <= 32 ? launch_split<void, 2>(a, glu, grouped, st) : launch_split<void, 1>(a, glu, grouped, st);
+    // The tiles add up in the same order, so that this one can take the place of those whose loads have 32-bit offsets without a bit's
+    // difference.
+    if (a.code_bytes == 0) return launch_gemm<2, 2, 3>(a, glu, grouped, st);
+    if (wide) return launch_gemm<4, 8, 1>(a, glu, grouped, st);
+    if (middle) return launch_gemm<2, 8, 1>(a, glu, grouped, st);
+    return narrow ? launch_gemm<2, 4, 1>(a, glu, grouped, st) : launch_gemm<2, 2, 3>(a, glu, grouped, st);
 }
 
 }  // namespace

@@ -93,3 +93,33 @@ def test_gates_far_below_zero(gpu, form, n, m):
     got = y.cpu().numpy().astype(np.float64)
     bad = (np.abs(got - want) > tol) & keep | ~keep & ~np.isinf(got)
     assert not bad.any(), [(g[c], u[c], got[r, c], want[c]) for r, c in np.argwhere(bad)[:5]]
+
+
+@pytest.mark.parametrize("n,k,m", [(2560, 6912, 24), (4864, 896, 48), (640, 2560, 30), (4096, 1024, 300), (2880, 2304, 700), (10240, 1024, 600)])
+def test_order_of_sums_by_shapes_alone(gpu, n, k, m):
+    """Operand rows that span 2^32 bytes give the bits of adjacent ones, on scales so wide apart that every sum rounds."""
+    import torch
+    torch.cuda.empty_cache()
+    g = torch.Generator(device="cuda").manual_seed(n + m)
+
+    def packed(*shape):
+        c = torch.randint(0, 256, (*shape, mx4_ref.kpad(k) // 2), dtype=torch.uint8, device="cuda", generator=g)
+        s = torch.randint(115, 140, (*shape, mx4_ref.kpad(k) // 32), dtype=torch.uint8, device="cuda", generator=g)
+        c[..., (k + 1) // 2:], s[..., -(-k // 32):] = 0, 0
+        return c, s
+
+    w = gpu.Mx4Weight(n, k, *packed(2, n), experts=2)
+    one = gpu.Mx4Weight(n, k, *packed(n))
+    codes, scales = packed(m)
+    stride = (5 << 30) // (m - 1) // 16 * 16
+    far = torch.empty(stride * (m - 1) + codes.shape[1], dtype=torch.uint8, device="cuda").as_strided(codes.shape, (stride, 1))
+    far.copy_(codes)
+    offsets = dev(np.array([0, m // 3, m], np.int32))
+    got = []
+    for c in (codes, far):
+        y = torch.full((2, m, n), float("nan"), device="cuda")
+        one.linear(c, scales, y[0])
+        w.linear_grouped(c, scales, offsets, y[1])
+        torch.cuda.synchronize()
+        got.append(y)
+    assert not got[0].isnan().any() and torch.equal(got[0], got[1])

@@ -77,3 +77,18 @@ def test_products_that_no_launch_holds(fake):  # noqa: F811
         assert launched() == grid
         lib.eif_hip_mx4_weight_destroy(h)
     """)
+
+
+def test_strides_do_not_change_the_order_of_sums(fake):  # noqa: F811
+    """Few rows that span 2^32 bytes take the form of adjacent ones, whose waves' partial sums meet in the same order."""
+    run(fake, LAUNCHED + """
+    for rows, cols, M in ((2560, 6912, 24), (4864, 896, 48), (64, 300, 300)):
+        rc, h = create(rows, cols)
+        kp, forms = lib.eif_hip_mx4_kpad(cols), []
+        for ldc in (kp // 2, 1 << 30):
+            fake.fake_reset()
+            assert rc == 0 and lib.eif_hip_mx4_linear(h, X, ldc, X, kp // 32, None, 0, X, rows, M, None) == 0
+            forms.append((launched(), fake.fake_launch_block(0)))
+        assert forms[0] == forms[1] and forms[0][1] == 512, (rows, cols, M, forms)
+        lib.eif_hip_mx4_weight_destroy(h)
+    """)
