@@ -838,13 +838,14 @@ int launch_quant(const void *x, int64_t ldx, int rows, int cols, uint8_t *codes,
     return EIF_HIP_OK;
 }
 
-// What every product checks: the weight, its device, the output and the gated form's rows.
-int check_product(const eif_hip_mx4_weight *w, int glu, const float *y, int64_t ldy, int M)
+// What every product checks: the weight, its device, the biases, the output and the gated form's rows.
+int check_product(const eif_hip_mx4_weight *w, const float *bias, int glu, const float *y, int64_t ldy, int M)
 {
     if (!w || M < 0) return EIF_HIP_E_ARG;
     if (M > kMaxRows) return EIF_HIP_E_LIMIT;
     if (glu && w->rows % 32 != 0) return EIF_HIP_E_LIMIT;
     if (ldy < (glu ? w->rows / 2 : w->rows) || (M > 0 && !y)) return EIF_HIP_E_ARG;
+    if (!aligned(y, 4) || !aligned(bias, 4)) return EIF_HIP_E_ARG;
     int dev = -1;
     if (hipGetDevice(&dev) != hipSuccess) return EIF_HIP_E_DEVICE;
     return dev == w->device ? EIF_HIP_OK : EIF_HIP_E_ARG;
@@ -1088,7 +1089,7 @@ int eif_hip_mx4_weight_info(const eif_hip_mx4_weight *w, int *experts, int *rows
 int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales, int64_t lds,
                        const float *bias, int glu, float *y, int64_t ldy, int M, void *stream)
 {
-    int rc = check_product(w, glu, y, ldy, M);
+    int rc = check_product(w, bias, glu, y, ldy, M);
     if (rc) return rc;
     if (w->experts != 1) return EIF_HIP_E_ARG;
     if (M == 0) return EIF_HIP_OK;
@@ -1102,7 +1103,7 @@ int eif_hip_mx4_linear(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_
 int eif_hip_mx4_linear_rows(const eif_hip_mx4_weight *w, const void *x, int type, int64_t ldx, const float *bias, int glu,
                             float *y, int64_t ldy, int M, void *stream)
 {
-    const int rc = check_product(w, glu, y, ldy, M);
+    const int rc = check_product(w, bias, glu, y, ldy, M);
     if (rc) return rc;
     if (w->experts != 1 || ldx < w->cols || type < EIF_HIP_F32 || type > EIF_HIP_BF16) return EIF_HIP_E_ARG;
     if (M > kRowsMaxM || w->cols > kRowsMaxCols) return EIF_HIP_E_LIMIT;
@@ -1120,7 +1121,7 @@ int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes
                                int64_t lds, int rows_in, const int32_t *row_index, const int32_t *offsets,
                                const float *bias, int glu, float *y, int64_t ldy, int M, void *stream)
 {
-    int rc = check_product(w, glu, y, ldy, M);
+    int rc = check_product(w, bias, glu, y, ldy, M);
     if (rc) return rc;
     if (rows_in < 0) return EIF_HIP_E_ARG;
     if (M == 0 || rows_in == 0) return EIF_HIP_OK;

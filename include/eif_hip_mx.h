@@ -12,7 +12,8 @@
  * one that the memory, the stream and the weight belong to (a product on another device than its weight's returns
  * EIF_HIP_E_ARG). Calls keep no memory between them besides the weights: any number of them may run at once, also on one
  * weight, and they may be captured into graphs (eif_hip_mx4_weight_create may not). Strides are in elements (codes and
- * scales: bytes). No input may overlap an output.
+ * scales: bytes). No input may overlap an output. Pointers are aligned to their elements where a call asks for no more, else
+ * EIF_HIP_E_ARG.
  */
 #ifndef EIF_HIP_MX_H
 #define EIF_HIP_MX_H

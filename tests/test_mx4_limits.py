@@ -92,3 +92,20 @@ def test_strides_do_not_change_the_order_of_sums(fake):  # noqa: F811
         assert forms[0] == forms[1] and forms[0][1] == 512, (rows, cols, M, forms)
         lib.eif_hip_mx4_weight_destroy(h)
     """)
+
+
+def test_misaligned_floats(fake):  # noqa: F811
+    run(fake, LAUNCHED + """
+    rc, h = create(64, 256)
+    def calls(bias, y, M=5):
+        fake.fake_reset()
+        return [lib.eif_hip_mx4_linear(h, X, 128, X, 8, bias, 0, y, 64, M, None),
+                lib.eif_hip_mx4_linear_rows(h, X, 0, 256, bias, 0, y, 64, M, None),
+                lib.eif_hip_mx4_linear_grouped(h, X, 128, X, 8, 5, X, X, bias, 0, y, 64, M, None)]
+    assert rc == 0 and calls(at(4), at(4)) == [0] * 3 and calls(None, at(12)) == [0] * 3
+    for n in (1, 2, 3):
+        assert calls(X, at(n)) == [ARG] * 3 and calls(at(n), X) == [ARG] * 3 and calls(at(n), X, 0) == [ARG] * 3
+        assert not launched()
+    assert lib.eif_hip_mx4_quant_rows(X, 0, 256, 2, 256, None, 0, None, 0, at(2), 256, None) == ARG
+    lib.eif_hip_mx4_weight_destroy(h)
+    """)
