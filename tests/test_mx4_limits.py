@@ -109,3 +109,12 @@ def test_misaligned_floats(fake):  # noqa: F811
     assert lib.eif_hip_mx4_quant_rows(X, 0, 256, 2, 256, None, 0, None, 0, at(2), 256, None) == ARG
     lib.eif_hip_mx4_weight_destroy(h)
     """)
+
+
+def test_info_of_no_weight(fake):  # noqa: F811
+    run(fake, LAUNCHED + """
+    assert lib.eif_hip_mx4_weight_info(None, None, None, None, None, None) == ARG
+    rc, h = create(64, 256)
+    assert rc == 0 and lib.eif_hip_mx4_weight_info(h, None, None, None, None, None) == 0
+    lib.eif_hip_mx4_weight_destroy(h)
+    """)
