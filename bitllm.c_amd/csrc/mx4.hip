@@ -1030,6 +1030,7 @@ int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, i
     hipStream_t st = (hipStream_t)stream;
     // host rows go up as they lie, up to the last row's end
     const size_t all = (size_t)experts * rows;
+    if (ldc > INT64_MAX / (int64_t)all || lds > INT64_MAX / (int64_t)all) return EIF_HIP_E_LIMIT;
     const size_t src_c = (all - 1) * ldc + ((size_t)cols + 1) / 2, src_s = (all - 1) * lds + ((size_t)cols + 31) / 32;
     uint8_t *up = nullptr;
     int rc = EIF_HIP_OK;

@@ -49,8 +49,9 @@ typedef struct eif_hip_mx4_weight eif_hip_mx4_weight;
 
 /* `experts` matrices [rows, cols] in the format above (row r of matrix e: codes + (e rows + r) ldc, ldc >=
  * (cols + 1) / 2; scales alike, lds >= (cols + 31) / 32; any alignment) -> the GPU layout, resident on the current device
- * until eif_hip_mx4_weight_destroy. Host pointers (src_on_device = 0) or device pointers (1). Synchronous. More than 4096
- * experts, 2^30 rows or 2^24 columns: EIF_HIP_E_LIMIT. */
+ * until eif_hip_mx4_weight_destroy. Host pointers (src_on_device = 0; the bytes between the rows are read too) or device pointers
+ * (1). Synchronous. More than 4096 experts, 2^30 rows, 2^24 columns or 2^31 - 1 tiles of 16 rows of all experts, or sources of
+ * 2^63 bytes and more: EIF_HIP_E_LIMIT. */
 int eif_hip_mx4_weight_create(eif_hip_mx4_weight **out, int experts, int rows, int cols, const uint8_t *codes,
                               int64_t ldc, const uint8_t *scales, int64_t lds, int src_on_device, void *stream);
 void eif_hip_mx4_weight_destroy(eif_hip_mx4_weight *w);

@@ -118,3 +118,17 @@ def test_info_of_no_weight(fake):  # noqa: F811
     assert rc == 0 and lib.eif_hip_mx4_weight_info(h, None, None, None, None, None) == 0
     lib.eif_hip_mx4_weight_destroy(h)
     """)
+
+
+def test_weight_sources_without_end(fake):  # noqa: F811
+    """Strides whose product with the rows passes 64 bits are refused before anything is allocated or copied."""
+    run(fake, LAUNCHED + """
+    h, n = vp(), fake.fake_mallocs()
+    src = np.zeros(1 << 16, np.uint8)
+    src = vp(src.ctypes.data)
+    for dev in (0, 1):
+        for experts, rows, ldc, lds in ((1, 5, 1 << 62, 2), (1, 5, 32, 1 << 62), (4096, 1 << 12, 1 << 40, 2), (1, 2, (1 << 63) - 1, 2)):
+            fake.fake_reset()
+            assert lib.eif_hip_mx4_weight_create(C.byref(h), experts, rows, 64, src, ldc, src, lds, dev, None) == LIMIT, (ldc, lds)
+            assert not launched() and not h.value and fake.fake_mallocs() == n
+    """)
