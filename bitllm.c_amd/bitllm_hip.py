@@ -309,6 +309,20 @@ def _row_type(t):
     return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
 
 
+def _device_tensor(t, name, dtypes, *least):
+    """A HipError unless t is a device tensor of one of `dtypes`, with as many dimensions as `least` and at least so much of each, its
+    last dimension contiguous."""
+    if not getattr(t, "is_cuda", False):
+        raise HipError(f"{name}: not a tensor on the device")
+    shape = tuple(t.shape)
+    if t.dtype not in dtypes:
+        raise HipError(f"{name}: {t.dtype}, not {' or '.join(map(str, dtypes))}")
+    if len(shape) != len(least) or any(n < m for n, m in zip(shape, least)):
+        raise HipError(f"{name}: {shape} is not at least {least}")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise HipError(f"{name}: elements of a row are not adjacent")
+
+
 def mx4_kpad(cols):
     return load().eif_hip_mx4_kpad(cols)
 
@@ -316,7 +330,14 @@ def mx4_kpad(cols):
 def mx4_quant_rows(x, codes=None, scales=None, values=None, stream=None):
     """Rows x [rows, cols] (device) -> MXFP4 codes [rows, >= kpad / 2] and scales [rows, >= kpad / 32] (uint8), and/or
     the float32 values they stand for."""
+    import torch
+    _device_tensor(x, "x", (torch.float32, torch.float16, torch.bfloat16), 0, 1)
     rows, cols = x.shape
+    kpad = mx4_kpad(cols)
+    for t, name, dtype, least in ((codes, "codes", torch.uint8, kpad // 2), (scales, "scales", torch.uint8, kpad // 32),
+                                  (values, "values", torch.float32, cols)):
+        if t is not None:
+            _device_tensor(t, name, (dtype,), rows, least)
     ld = lambda t: 0 if t is None else t.stride(0)   # noqa: E731
     check(load().eif_hip_mx4_quant_rows(ptr(x), _row_type(x), ld(x), rows, cols, ptr(codes), ld(codes), ptr(scales),
                                         ld(scales), ptr(values), ld(values), stream_ptr(stream)),
@@ -333,17 +354,21 @@ class Mx4Weight:
         if on_device != hasattr(scales, "data_ptr"):
             raise HipError("Mx4Weight: codes and scales are both on the device or both on the host")
 
-        def row_stride(t):
+        def row_stride(t, least):
+            if on_device and not t.is_cuda or str(t.dtype).split(".")[-1] != "uint8":
+                raise HipError("Mx4Weight: codes and scales are uint8, torch tensors on the device or numpy arrays")
             s = [t.stride(i) if on_device else t.strides[i] for i in range(len(t.shape))]
             if t.shape != ((experts, rows, t.shape[-1]) if len(s) == 3 else (experts * rows, t.shape[-1])) or s[-1] != 1:
                 raise HipError(f"Mx4Weight: {tuple(t.shape)} is not {experts} x {rows} rows of bytes")
             if len(s) == 3 and experts > 1 and s[0] != rows * s[1]:
                 raise HipError("Mx4Weight: the matrices' rows are not evenly spaced")
+            if t.shape[-1] < least:
+                raise HipError(f"Mx4Weight: rows of {t.shape[-1]} bytes for {cols} columns, {least} at least")
             return s[-2]
 
         h = C.c_void_p()
-        check(lib.eif_hip_mx4_weight_create(C.byref(h), experts, rows, cols, ptr(codes), row_stride(codes), ptr(scales),
-                                            row_stride(scales), 1 if on_device else 0,
+        check(lib.eif_hip_mx4_weight_create(C.byref(h), experts, rows, cols, ptr(codes), row_stride(codes, (cols + 1) // 2),
+                                            ptr(scales), row_stride(scales, (cols + 31) // 32), 1 if on_device else 0,
                                             stream_ptr(stream) if on_device else None), "eif_hip_mx4_weight_create")
         self.h, self.rows, self.cols, self.experts = h, rows, cols, experts
         k, b = C.c_int(), C.c_size_t()
@@ -361,19 +386,40 @@ class Mx4Weight:
         except Exception:
             pass
 
+    def _check(self, y, m, bias, glu, codes=None, scales=None, rows_in=0):
+        import torch
+        _device_tensor(y, "y", (torch.float32,), m, self.rows // 2 if glu else self.rows)
+        if bias is not None:
+            _device_tensor(bias, "bias", (torch.float32,), *((self.experts, self.rows) if len(bias.shape) == 2 else (self.experts * self.rows,)))
+            if len(bias.shape) == 2 and self.experts > 1 and bias.stride(0) != self.rows:
+                raise HipError("bias: the matrices' biases are not adjacent")
+        if codes is not None:
+            _device_tensor(codes, "codes", (torch.uint8,), rows_in, self.kpad // 2)
+            _device_tensor(scales, "scales", (torch.uint8,), rows_in, self.kpad // 32)
+
     def linear(self, codes, scales, y, bias=None, glu=False, stream=None):
         """y [M, rows or rows / 2] = the product of M quantised rows (mx4_quant_rows)."""
+        self._check(y, y.shape[0], bias, glu, codes, scales, y.shape[0])
         check(load().eif_hip_mx4_linear(self.h, ptr(codes), codes.stride(0), ptr(scales), scales.stride(0), ptr(bias),
                                         int(glu), ptr(y), y.stride(0), y.shape[0], stream_ptr(stream)),
               "eif_hip_mx4_linear")
 
     def linear_rows(self, x, y, bias=None, glu=False, stream=None):
         """The same for M <= 8 unquantised rows x, quantised within the launch."""
+        import torch
+        _device_tensor(x, "x", (torch.float32, torch.float16, torch.bfloat16), 0, self.cols)
+        self._check(y, x.shape[0], bias, glu)
         check(load().eif_hip_mx4_linear_rows(self.h, ptr(x), _row_type(x), x.stride(0), ptr(bias), int(glu), ptr(y),
                                              y.stride(0), x.shape[0], stream_ptr(stream)), "eif_hip_mx4_linear_rows")
 
     def linear_grouped(self, codes, scales, offsets, y, row_index=None, bias=None, glu=False, stream=None):
-        """Rows [offsets[e], offsets[e + 1]) of y take matrix e; row i takes the quantised row row_index[i] (None: i)."""
+        """Rows [offsets[e], offsets[e + 1]) of y take matrix e; row i takes the quantised row row_index[i] (None: i). offsets
+        [experts + 1] and row_index [y's rows] are int32, on the device."""
+        import torch
+        self._check(y, y.shape[0], bias, glu, codes, scales, codes.shape[0])
+        _device_tensor(offsets, "offsets", (torch.int32,), self.experts + 1)
+        if row_index is not None:
+            _device_tensor(row_index, "row_index", (torch.int32,), y.shape[0])
         check(load().eif_hip_mx4_linear_grouped(self.h, ptr(codes), codes.stride(0), ptr(scales), scales.stride(0),
                                                 codes.shape[0], ptr(row_index), ptr(offsets), ptr(bias), int(glu), ptr(y),
                                                 y.stride(0), y.shape[0], stream_ptr(stream)),

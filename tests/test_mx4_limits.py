@@ -132,3 +132,94 @@ def test_weight_sources_without_end(fake):  # noqa: F811
             assert lib.eif_hip_mx4_weight_create(C.byref(h), experts, rows, 64, src, ldc, src, lds, dev, None) == LIMIT, (ldc, lds)
             assert not launched() and not h.value and fake.fake_mallocs() == n
     """)
+
+
+TENSORS = LAUNCHED + """
+    import torch
+
+    class T:
+        \"\"\"A device tensor as far as the binding looks at one.\"\"\"
+        def __init__(self, *shape, dtype=torch.float32, strides=None, cuda=True):
+            self.shape, self.dtype, self.is_cuda = torch.Size(shape), dtype, cuda
+            self.strides_ = strides or [int(np.prod(shape[i + 1:])) for i in range(len(shape))]
+        def stride(self, i):
+            return self.strides_[i]
+        def data_ptr(self):
+            return X.value
+
+    class S:
+        cuda_stream = 0
+
+    u8, i32, i64, f16, f64 = torch.uint8, torch.int32, torch.int64, torch.float16, torch.float64
+
+    def refused(f, *args, **kw):
+        fake.fake_reset()
+        try:
+            f(*args, stream=S, **kw)
+        except bh.HipError as e:
+            return not launched() and "(-" not in str(e)   # by the binding, not by the library
+        return False
+
+    def taken(f, *args, **kw):
+        fake.fake_reset()
+        f(*args, stream=S, **kw)
+        return len(launched()) == 1
+"""
+
+
+def test_binding_quant_rows(fake):  # noqa: F811
+    run(fake, TENSORS + """
+    q, x, c, s, v = bh.mx4_quant_rows, T(5, 300), T(5, 256, dtype=u8), T(5, 16, dtype=u8), T(5, 300)
+    assert taken(q, x, c, s, v) and taken(q, x, c, s) and taken(q, x, values=v) and taken(q, T(5, 300, dtype=f16), T(7, 272, dtype=u8), s)
+    for args in ((T(5, 300, cuda=False), c, s), (torch.zeros(5, 300), c, s), (T(5, 300, dtype=f64), c, s), (T(5, 300, strides=[1, 5]), c, s),
+                 (T(300), c, s), (x, T(4, 256, dtype=u8), s), (x, T(5, 240, dtype=u8), s), (x, T(5, 256, dtype=i32), s),
+                 (x, c, T(4, 16, dtype=u8)), (x, c, T(5, 8, dtype=u8)), (x, c, T(5, 16)), (x, c, s, T(4, 300)), (x, c, s, T(5, 299)),
+                 (x, c, s, T(5, 300, dtype=f16)), (x, c, s, T(5, 300, cuda=False)), (x, c, s, T(5, 300, strides=[900, 3]))):
+        assert refused(q, *args), [(t.shape, t.dtype) for t in args]
+    """)
+
+
+def test_binding_weight(fake):  # noqa: F811
+    run(fake, TENSORS + """
+    def W(c, s, experts=1, stream=None):
+        return bh.Mx4Weight(64, 300, c, s, experts=experts, stream=S)
+    for c, s, e in ((T(64, 150, dtype=u8), T(64, 10, dtype=u8), 1), (T(2, 64, 160, dtype=u8), T(2, 64, 10, dtype=u8), 2),
+                    (np.zeros((64, 150), np.uint8), np.zeros((64, 10), np.uint8), 1)):
+        W(c, s, e).close()
+    c, s = T(64, 150, dtype=u8), T(64, 10, dtype=u8)
+    for args in ((T(64, 150, dtype=u8, cuda=False), s), (c, T(64, 10, dtype=u8, cuda=False)), (torch.zeros(64, 150, dtype=u8), torch.zeros(64, 10, dtype=u8)),
+                 (T(64, 150, dtype=i32), s), (c, T(64, 10)), (T(64, 149, dtype=u8, strides=[160, 1]), s), (c, T(64, 9, dtype=u8, strides=[16, 1])),
+                 (T(63, 150, dtype=u8), s), (c, np.zeros((64, 10), np.uint8)), (np.zeros((64, 150), np.int8), np.zeros((64, 10), np.uint8))):
+        assert refused(W, *args), args
+    """)
+
+
+def test_binding_products(fake):  # noqa: F811
+    """Tensors that a product would read or write beyond their ends, or take for another type, never reach it."""
+    run(fake, TENSORS + """
+    w, g = mx4(64, 300), mx4(64, 300, 3)
+    c, s, y, h = T(5, 256, dtype=u8), T(5, 16, dtype=u8), T(5, 64), T(5, 32)
+    off, idx, b, bg = T(4, dtype=i32), T(5, dtype=i32), T(64), T(3, 64)
+    lin, rows, grp = w.linear, w.linear_rows, lambda c, s, y, **k: g.linear_grouped(c, s, k.pop("off", off), y, **k)
+    for f in (lin, grp):
+        ok = b if f is lin else bg
+        assert taken(f, c, s, y) and taken(f, c, s, y, bias=ok) and taken(f, c, s, h, glu=True) and taken(f, T(9, 272, dtype=u8), T(9, 24, dtype=u8), y)
+        bad = [(T(5, 240, dtype=u8), s, y), (c, T(5, 8, dtype=u8), y), (c, T(4, 16, dtype=u8), y), (T(5, 256, dtype=i32), s, y), (c, T(5, 16), y),
+               (T(5, 256, dtype=u8, cuda=False), s, y), (c, s, T(5, 63)), (c, s, T(5, 64, dtype=f16)), (c, s, T(5, 64, cuda=False)),
+               (c, s, T(5, 64, strides=[1, 5])), (c, s, T(64))]
+        for args in bad + ([(T(4, 256, dtype=u8), s, y)] if f is lin else []):
+            assert refused(f, *args), [(t.shape, t.dtype) for t in args]
+        assert refused(f, c, s, T(5, 31), glu=True)
+    for bias in (T(63), T(64, dtype=f16), T(64, cuda=False), T(64, strides=[2])):
+        assert refused(lin, c, s, y, bias=bias) and refused(rows, T(5, 300), y, bias=bias)
+    for bias in (b, T(2, 64), T(3, 63), T(3, 64, strides=[80, 1]), T(191), T(3, 64, dtype=f16)):
+        assert refused(grp, c, s, y, bias=bias)
+    assert taken(grp, c, s, y, bias=T(192)) and taken(grp, c, s, y, row_index=idx) and taken(grp, T(2, 256, dtype=u8), T(2, 16, dtype=u8), y)
+    for o in (T(4, dtype=i64), T(3, dtype=i32), T(4, dtype=i32, strides=[2]), T(4, dtype=i32, cuda=False)):
+        assert refused(grp, c, s, y, off=o)
+    for i in (T(5, dtype=i64), T(4, dtype=i32), T(5, dtype=i32, strides=[2]), T(5, dtype=i32, cuda=False)):
+        assert refused(grp, c, s, y, row_index=i)
+    assert taken(rows, T(5, 300), y) and taken(rows, T(3, 304, dtype=f16), y) and taken(rows, T(5, 300), h, glu=True)
+    for args in ((T(6, 300), y), (T(5, 299), y), (T(5, 300, dtype=f64), y), (T(5, 300, cuda=False), y), (T(5, 300, strides=[1, 5]), y), (T(5, 300), T(5, 63))):
+        assert refused(rows, *args), [(t.shape, t.dtype) for t in args]
+    """)
