@@ -123,3 +123,39 @@ def test_order_of_sums_by_shapes_alone(gpu, n, k, m):
         torch.cuda.synchronize()
         got.append(y)
     assert not got[0].isnan().any() and torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("n,m", [(96, 3), (96, 40), (4096, 300), (4130, 1100)])
+def test_scale_bytes_of_the_whole_range(gpu, n, m):
+    """Scale bytes that the quantiser never gives, 253 and 254, against 1 and 0: the scales' products are 1, the sums exact."""
+    import torch
+    k = 1024
+    rng = np.random.default_rng(n + m)
+    byte = rng.choice([0, 1, 2, 127, 252, 253, 254], k // 32).astype(np.uint8)
+    wc, ac = (dev(rng.integers(0, 256, (r, k // 2)).astype(np.uint8)) for r in (n, m))
+    w = gpu.Mx4Weight(n, k, wc, dev(np.tile(byte, (n, 1))))
+    y = torch.full((m, n), float("nan"), device="cuda")
+    w.linear(ac, dev(np.tile(254 - byte, (m, 1)).astype(np.uint8)), y)
+    torch.cuda.synchronize()
+    one = np.full(k // 32, 127, np.uint8)
+    want = mx4_ref.values(ac.cpu().numpy(), np.tile(one, (m, 1)), k) @ mx4_ref.values(wc.cpu().numpy(), np.tile(one, (n, 1)), k).T
+    assert np.array_equal(y.cpu().numpy().astype(np.float64), want)
+
+
+def test_one_row_of_many_experts(gpu):
+    """One row to the last of 4096 matrices, and none to any."""
+    import torch
+    experts, n, k = 4096, 48, 64
+    rng = np.random.default_rng(3)
+    wc, ws = mx4_ref.quantise(mx4_ref.matrix(rng, experts * n, k))
+    wc, ws = wc[:, :k // 2], ws[:, :k // 32]
+    w = gpu.Mx4Weight(n, k, dev(wc).reshape(experts, n, -1), dev(ws).reshape(experts, n, -1), experts=experts)
+    ac, as_ = mx4_ref.quantise(mx4_ref.activations(rng, 2, k))
+    want, tol = mx4_ref.product(mx4_ref.values(ac, as_, k)[1:], mx4_ref.values(wc[-n:], ws[-n:], k))
+    for last in (1, 0):
+        offsets = np.zeros(experts + 1, np.int32)
+        offsets[-1] = last
+        y = torch.full((1, n), float("nan"), device="cuda")
+        w.linear_grouped(dev(ac), dev(as_), dev(offsets), y, dev(np.array([1], np.int32)))
+        torch.cuda.synchronize()
+        assert (np.abs(y.cpu().numpy() - want) <= tol).all() if last else y.isnan().all()
