@@ -915,8 +915,10 @@ int launch_split_deep(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
     const int n = eif_ceil_div(a.spans, KW);   // spans of a wave
     if (n == 1) return launch_split_as<X, TT, KW, 1>(a, glu, grouped, st);
-    if (n == 2 || TT > 1) return launch_split_as<X, TT, KW, 2>(a, glu, grouped, st);
-    return launch_split_as<X, TT, KW, TT == 1 ? 4 : 2>(a, glu, grouped, st);
+    if constexpr (TT == 1) {
+        if (n > 2) return launch_split_as<X, TT, KW, 4>(a, glu, grouped, st);
+    }
+    return launch_split_as<X, TT, KW, 2>(a, glu, grouped, st);
 }
 
 // Waves that share a row tile: as many as keep the launch at 4096 row tiles times waves, 4 a SIMD (the rows form: 3500; each
