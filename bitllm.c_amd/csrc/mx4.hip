@@ -108,8 +108,9 @@ EIF_DEV uint32_t quantise4(const float *v, uint32_t &byte)
 
 // One wave a row and span: lane l has columns 4 l .. 4 l + 3, a block is eight lanes, and a wave's loads and stores are one run.
 // Bound by memory: 3001x6912 FP32 with values 34.3 us, 5.2 TB/s of what it reads and writes (43 with values stored four bytes at
-// a time); without values 17.7, 5.3 TB/s. Two to eight spans a wave, their loads first, were no faster (34.0 to 37.6) and small
-// calls slower (64x2560 2.1 us with one, 2.5 with two).
+// a time); without values 20.6, 4.6 TB/s. Two to eight spans a wave, their loads first, were no faster (34.0 to 37.6) and small
+// calls slower (64x2560 2.1 us with one, 2.5 with two). Not so 2-byte rows without values: 13824x2560 28.8 us (bf16) and 29.8 (f16),
+// 3.0 TB/s, hardly less than the 34.0 of FP32 rows; there the waves' instructions count (all on inputs of more than 512 MB in turn).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T *x, int64_t ldx, int rows, int cols, int spans,
                                                          uint8_t *codes, int64_t ldc, uint8_t *scales, int64_t lds,
@@ -504,7 +505,7 @@ EIF_DEV void load_lds16(__amdgpu_buffer_rsrc_t src, uint32_t lane_offset, uint32
 // whole cache lines; row n's piece h lies at place 8 (n % 8) + (h ^ place(n)) of its half of the tile. LDS takes a read of
 // 16 bytes a lane 16 lanes at a time, rows 0-3 and 12-15 of one slot with rows 4-11 of the next; place() gives them 16
 // different groups of banks (with n / 2 in its place they met in pairs).
-//   What bounds it: 4096 rows through 8192x8192 take 126 to 133 us, 4.1 to 4.4 PFLOP/s; the matrix instructions alone run at 7.1 here (at
+//   What bounds it: 4096 rows through 8192x8192 take 126 to 136 us, 4.0 to 4.4 PFLOP/s; the matrix instructions alone run at 7.1 here (at
 // 1.7 GHz, where power holds them), and the 134 MB of outputs take 28 us of it. A span of the two workgroups on a CU is 2048
 // cycles of matrix instructions, and L2 has to bring 96 KB meanwhile. (Before whole-line loads of token rows and scales by
 // pairs of spans its request rate was the bound: 271 us. Tiles of 256x256 rows with eight waves took 5 % longer, a workgroup
@@ -922,7 +923,8 @@ int launch_split_deep(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 }
 
 // Waves that share a row tile: as many as keep the launch at 4096 row tiles times waves, 4 a SIMD (the rows form: 3500; each
-// workgroup quantises the rows, and more waves a tile are more workgroups). Measured (us, 1 / 2 / 4 / 8 waves): one row, 151936x1024
+// workgroup quantises the rows, and more waves a tile are more workgroups). Measured on three sets of inputs in turn, which the
+// Infinity Cache holds whole or in part (us, 1 / 2 / 4 / 8 waves): one row, 151936x1024
 // 13.9 / 14.1 / 15.2 / 23.1; 8 rows, 8192x8192 19.8 / 11.9 / 9.2 / 8.7, gated 13824x2560 in the rows form 11.0 / 9.8 /
 // 9.2 / 11.0; 32 rows by expert, about 22 experts of gated 2816x2560 13.6 / 18.1 / 19.4 / 17.2.
 template <typename X, int TT>
@@ -963,15 +965,17 @@ int launch_gemm(Mx4Args a, bool glu, bool grouped, hipStream_t st)
 }
 
 // The form of a product of quantised rows: the largest tile that still gives the 256 CUs workgroups enough (200; 256; 160); of a few
-// rows the split form. By expert a tile of more token rows than an expert has on average is mostly empty. Measured (us; 256
+// rows the split form. By expert a tile of more token rows than an expert has on average is mostly empty. The limits are set by
+// these measurements, within 6 % of the best form but for 800 rows through 5120x5120 (23.4, where 256x128 takes 20.8). Measured (us; 256
 // rows x 128 tokens / 128x128 / 128x64 / 128x32 three spans ahead / split; in brackets the workgroups of the first three):
 //   4096 rows, 8192x8192 133 / 149 / 187 / 291 / 1615 (1024, 2048, 4096); 512, gated 13824x2560 15.0 / 16.2 / 18.5 / 25.1 / 87 (216,
 //   432, 864); 800, 5120x5120 20.8 / 23.4 / 23.3 / 26.1 / - (140, 280, 520); 1024, 4096x4096 17.6 / 14.2 / 14.9 / 21.6 / 103 (128,
-//   256, 512); 1500, 2560x2560 13.3 / 10.3 / 10.3 / 15.7 / - (120, 240, 480); 384, 8192x8192 29 / 21 / 22 / 29 / - (96, 192,
-//   384); 640, 2560x6912 26 / 18.3 / 15.2 / 18.0 / - (50, 100, 200); 128, 8192x8192 29 / 20 / 16.9 / 13.8 / 53 (32, 64, 128); 256,
+//   256, 512); 1500, 2560x2560 13.3 / 10.3 / 10.3 / 15.7 / - (120, 240, 480); 384, 8192x8192 29 / 21 / 22 / 29 / - (96, 192, 384);
+//   640, 2560x6912 26 / 18.3 / 15.2 / 18.0 / - (50, 100, 200); 128, 8192x8192 29 / 20 / 16.9 / 13.8 / 53 (32, 64, 128); 256,
 //   2560x6912 26 / 18.1 / 14.8 / 12.1 / 37 (20, 40, 80); 100, 2560x2560 12.1 / 8.1 / 6.0 / 6.3 / 10.3; 32, 8192x8192 28 / 19 / 16 /
-//   13.5 / 15.5; 600, 1024x1024 - / - / 4.3 / 4.2 / 8.2; 60, 4096x1024 - / - / 4.1 / 3.9 / 3.6; 48, 4864x896 7.4 / 5.2 / 4.0 / 4.0 / 3.6; 24, 2560x6912 24 / 16 / 14 / 11.6 / 6.1; by expert, gated 2816 rows: 16384
-//   rows to 64 99 / 113 / 121 / 163 / 389, 800 to 32 37 / 36 / 30 / 36 / 38; 2048 to 32 of 2048x1408 18.7 / 18.0 / 15.3 / 18.6 / 54.
+//   13.5 / 15.5; 600, 1024x1024 - / - / 4.3 / 4.2 / 8.2; 60, 4096x1024 - / - / 4.1 / 3.9 / 3.6; 48, 4864x896 7.4 / 5.2 / 4.0 / 4.0 /
+//   3.6; 24, 2560x6912 24 / 16 / 14 / 11.6 / 6.1; by expert, gated 2816 rows: 16384 rows to 64 99 / 113 / 121 / 163 / 389, 800 to 32
+//   37 / 36 / 30 / 36 / 38; 2048 to 32 of 2048x1408 18.7 / 18.0 / 15.3 / 18.6 / 54.
 int launch_product(const Mx4Args &a, bool glu, bool grouped, hipStream_t st)
 {
     const int m = grouped ? (a.M - 1) / a.experts + 1 : a.M;   // token rows of a matrix

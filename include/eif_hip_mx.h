@@ -11,9 +11,9 @@
  * stream), calls are asynchronous on it and return 0 or a negative EIF_HIP_E_* code. The current device must be the
  * one that the memory, the stream and the weight belong to (a product on another device than its weight's returns
  * EIF_HIP_E_ARG). Calls keep no memory between them besides the weights: any number of them may run at once, also on one
- * weight, and they may be captured into graphs (eif_hip_mx4_weight_create may not). Strides are in elements (codes and
- * scales: bytes). No input may overlap an output. Pointers are aligned to their elements where a call asks for no more, else
- * EIF_HIP_E_ARG.
+ * weight, and they may be captured into graphs (eif_hip_mx4_weight_create and _destroy, which allocate and free, may not).
+ * Strides are in elements (codes and scales: bytes). No input may overlap an output. Pointers are aligned to their elements
+ * where a call asks for no more, else EIF_HIP_E_ARG.
  */
 #ifndef EIF_HIP_MX_H
 #define EIF_HIP_MX_H
@@ -82,8 +82,9 @@ int eif_hip_mx4_linear_rows(const eif_hip_mx4_weight *w, const void *x, int type
  * [experts, rows] or NULL, and glu as above). offsets [experts + 1] int32 in device memory, non-decreasing, taken as if
  * cut to [0, M]; experts may have no rows. Row i of y takes the quantised row row_index[i] (int32 in device memory; NULL:
  * i) of `rows_in` rows. Rows of y before offsets[0] and from offsets[experts] on, and rows whose index is not in
- * [0, rows_in), are left as they were. (Where offsets decrease, so that ranges overlap, it is open which
- * of their rows are written, and with whose products.) */
+ * [0, rows_in), are left as they were. The form goes by M / experts, since the host does not see the offsets: up to 16 rows an
+ * expert on average read a matrix once for every 16 rows that it has, which is slow where many rows meet in one expert.
+ * (Where offsets decrease, so that ranges overlap, it is open which of their rows are written, and with whose products.) */
 int eif_hip_mx4_linear_grouped(const eif_hip_mx4_weight *w, const uint8_t *codes, int64_t ldc, const uint8_t *scales,
                                int64_t lds, int rows_in, const int32_t *row_index, const int32_t *offsets,
                                const float *bias, int glu, float *y, int64_t ldy, int M, void *stream);
