@@ -390,7 +390,8 @@ class Mx4Weight:
         import torch
         _device_tensor(y, "y", (torch.float32,), m, self.rows // 2 if glu else self.rows)
         if bias is not None:
-            _device_tensor(bias, "bias", (torch.float32,), *((self.experts, self.rows) if len(bias.shape) == 2 else (self.experts * self.rows,)))
+            least = (self.experts, self.rows) if len(bias.shape) == 2 else (self.experts * self.rows,)
+            _device_tensor(bias, "bias", (torch.float32,), *least)
             if len(bias.shape) == 2 and self.experts > 1 and bias.stride(0) != self.rows:
                 raise HipError("bias: the matrices' biases are not adjacent")
         if codes is not None:
