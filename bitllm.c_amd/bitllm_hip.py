@@ -24,6 +24,12 @@ class PrepSpec(C.Structure):
                 ("wht_block", _i), ("wht_norm", _f)]
 
 
+class MoeRouteSpec(C.Structure):
+    """eif_hip_moe_route_spec (include/eif_hip_moe.h)."""
+    _fields_ = [("experts", _i), ("top_k", _i), ("score", _i), ("bias", _vp), ("groups", _i), ("groups_kept", _i), ("group_best", _i),
+                ("renormalise", _i), ("scale", _f)]
+
+
 class BitnetConfig(C.Structure):
     """eif_hip_bitnet_config (include/eif_hip_decode.h)."""
     _fields_ = [(n, _i) for n in ("dim", "hidden", "n_layers", "n_heads", "n_kv_heads", "head_dim", "vocab", "seq_len")] + \
@@ -71,6 +77,15 @@ _SIGS = {
     "eif_hip_mx4_linear": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i, _vp, _i64, _i, _vp]),
     "eif_hip_mx4_linear_rows": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i64, _i, _vp]),
     "eif_hip_mx4_linear_grouped": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
+    "eif_hip_moe_sort_bytes": (_sz, [_i, _i, _i]),
+    "eif_hip_moe_route": (_i, [_vp, _i, _i64, _i, C.POINTER(MoeRouteSpec), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "eif_hip_moe_sort": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "eif_hip_moe_combine": (_i, [_vp, _i64, _i, _vp, _vp, _i, _i, _vp, _i64, _i, _vp, _i, _i64, _vp]),
+    "eif_hip_adapters_create": (_i, [C.POINTER(_vp), _i, _i, _i, _i, _i]),
+    "eif_hip_adapters_destroy": (None, [_vp]),
+    "eif_hip_adapters_set": (_i, [_vp, _i, _i, _vp, _i64, _vp, _i64, _f, _i, _vp]),
+    "eif_hip_adapters_info": (_i, [_vp] + [C.POINTER(_i)] * 5 + [C.POINTER(_sz)]),
+    "eif_hip_adapters_linear": (_i, [_vp, _vp, _i, _i64, _vp, _vp, _i64, _vp, _i64, _i, _vp]),
     "eif_gguf_ternary_rows": (_i, [_i, _vp, _i, _i, _vp, _vp]),
     "eif_hip_qweight_from_gguf_ternary": (_i, [_vp, _i, _vp, _i, _i, _vp]),
     "eif_hip_bitnet_create": (_i, [C.POINTER(_vp), C.POINTER(BitnetConfig)]),
@@ -425,6 +440,138 @@ class Mx4Weight:
                                                 codes.shape[0], ptr(row_index), ptr(offsets), ptr(bias), int(glu), ptr(y),
                                                 y.stride(0), y.shape[0], stream_ptr(stream)),
               "eif_hip_mx4_linear_grouped")
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1   # include/eif_hip_moe.h
+
+
+def _ints(t, name, n):
+    """A HipError unless t is a contiguous int32 tensor on the device of at least n elements."""
+    import torch
+    if not getattr(t, "is_cuda", False) or t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+        raise HipError(f"{name}: not {n} adjacent int32 on the device")
+
+
+def _sorted_outputs(offsets, row, slot, work, pairs, tokens, top_k, experts):
+    for t, name, n in ((offsets, "offsets", experts + 1), (row, "row", pairs), (slot, "slot", pairs)):
+        _ints(t, name, n)
+    if work is not None and not (work.is_cuda and work.is_contiguous()):
+        raise HipError("work: not a contiguous tensor on the device")
+    return ptr(offsets), ptr(row), ptr(slot), ptr(work), 0 if work is None else work.numel() * work.element_size()
+
+
+def moe_sort_bytes(tokens, top_k, experts):
+    return load().eif_hip_moe_sort_bytes(tokens, top_k, experts)
+
+
+def moe_route(logits, ids, weights, score=SCORE_SOFTMAX, bias=None, groups=1, groups_kept=1, group_best=1, renormalise=True, scale=1.0,
+              offsets=None, row=None, slot=None, work=None, stream=None):
+    """Logits [tokens, experts] (device) -> ids [tokens, top_k] int32 and weights [tokens, top_k] float32, and where offsets, row and
+    slot are given the pairs sorted by expert (moe_sort), with a workspace of moe_sort_bytes."""
+    import torch
+    _device_tensor(logits, "logits", (torch.float32, torch.float16, torch.bfloat16), 0, 1)
+    tokens, experts = logits.shape
+    _device_tensor(ids, "ids", (torch.int32,), tokens, 1)
+    top_k = ids.shape[1]
+    _device_tensor(weights, "weights", (torch.float32,), tokens, top_k)
+    if not ids.is_contiguous() or not weights.is_contiguous() or weights.shape[1] != top_k:
+        raise HipError("ids, weights: rows of top_k adjacent elements")
+    if bias is not None:
+        _device_tensor(bias, "bias", (torch.float32,), experts)
+    places = (None, None, None, None, 0)
+    if offsets is not None or row is not None or slot is not None:
+        places = _sorted_outputs(offsets, row, slot, work, tokens * top_k, tokens, top_k, experts)
+    spec = MoeRouteSpec(experts=experts, top_k=top_k, score=score, bias=None if bias is None else bias.data_ptr(), groups=groups,
+                        groups_kept=groups_kept, group_best=group_best, renormalise=int(renormalise), scale=scale)
+    check(load().eif_hip_moe_route(ptr(logits), _row_type(logits), logits.stride(0), tokens, C.byref(spec), ptr(ids), ptr(weights),
+                                   *places, stream_ptr(stream)), "eif_hip_moe_route")
+
+
+def moe_sort(ids, experts, offsets, row, slot, work=None, stream=None):
+    """Chosen experts ids [tokens, top_k] int32 (device) -> offsets [experts + 1], row and slot [tokens * top_k] int32."""
+    import torch
+    _device_tensor(ids, "ids", (torch.int32,), 0, 1)
+    if not ids.is_contiguous():
+        raise HipError("ids: rows of top_k adjacent elements")
+    tokens, top_k = ids.shape
+    places = _sorted_outputs(offsets, row, slot, work, tokens * top_k, tokens, top_k, experts)
+    check(load().eif_hip_moe_sort(ptr(ids), tokens, top_k, experts, *places, stream_ptr(stream)), "eif_hip_moe_sort")
+
+
+def moe_combine(y, slot, out, weights=None, add=None, stream=None):
+    """out [tokens, dim] = add + the sum over k of weights[t, k] y[slot[t, k]]; y [rows, dim] float32, slot [tokens, top_k] int32."""
+    import torch
+    _device_tensor(out, "out", (torch.float32, torch.float16, torch.bfloat16), 0, 1)
+    tokens, dim = out.shape
+    _device_tensor(y, "y", (torch.float32,), 0, dim)
+    _device_tensor(slot, "slot", (torch.int32,), tokens, 1)
+    top_k = slot.shape[1]
+    if not slot.is_contiguous():
+        raise HipError("slot: rows of top_k adjacent elements")
+    if weights is not None:
+        _device_tensor(weights, "weights", (torch.float32,), tokens, top_k)
+        if not weights.is_contiguous() or weights.shape[1] != top_k:
+            raise HipError("weights: rows of top_k adjacent elements")
+    if add is not None:
+        _device_tensor(add, "add", (torch.float32,), tokens, dim)
+    check(load().eif_hip_moe_combine(ptr(y), y.stride(0), y.shape[0], ptr(slot), ptr(weights), tokens, top_k, ptr(add),
+                                     0 if add is None else add.stride(0), dim, ptr(out), _row_type(out), out.stride(0),
+                                     stream_ptr(stream)), "eif_hip_moe_combine")
+
+
+class Adapters:
+    """Low-rank adapters of one projection [rows, cols], resident in HBM, `slots` of them at once (include/eif_hip_adapters.h)."""
+
+    def __init__(self, slots, rows, cols, max_rank, dtype):
+        import torch
+        h = C.c_void_p()
+        kinds = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        if dtype not in kinds:
+            raise HipError(f"Adapters: {dtype}, not float32, float16 or bfloat16")
+        check(load().eif_hip_adapters_create(C.byref(h), slots, rows, cols, max_rank, kinds[dtype]), "eif_hip_adapters_create")
+        self.h, self.slots, self.rows, self.cols, self.max_rank, self.dtype = h, slots, rows, cols, max_rank, dtype
+        b = C.c_size_t()
+        check(load().eif_hip_adapters_info(h, None, None, None, None, None, C.byref(b)), "eif_hip_adapters_info")
+        self.bytes = b.value
+
+    def close(self):
+        if self.h:
+            load().eif_hip_adapters_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set(self, slot, A, B, scale=1.0, stream=None):
+        """A [rank, cols] and B [rows, rank] (torch tensors of the adapters' type, both on the device or both on the host) into a slot."""
+        rank = A.shape[0]
+        for t, name, shape in ((A, "A", (rank, self.cols)), (B, "B", (self.rows, rank))):
+            if tuple(t.shape) != shape or t.dtype != self.dtype or (shape[1] > 1 and t.stride(1) != 1):
+                raise HipError(f"{name}: {tuple(t.shape)} {t.dtype}, not {shape} {self.dtype} with adjacent elements")
+        if A.is_cuda != B.is_cuda:
+            raise HipError("Adapters.set: A and B are both on the device or both on the host")
+        ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]   # noqa: E731
+        check(load().eif_hip_adapters_set(self.h, slot, rank, ptr(A), ld(A), ptr(B), ld(B), scale, int(A.is_cuda),
+                                          stream_ptr(stream)), "eif_hip_adapters_set")
+
+    def clear(self, slot, stream=None):
+        check(load().eif_hip_adapters_set(self.h, slot, 0, None, 0, None, 0, 0.0, 1, stream_ptr(stream)), "eif_hip_adapters_set")
+
+    def linear(self, x, slot, y, base=None, stream=None):
+        """y [M, rows] = base + the adapters' products of x [M, cols], row m's in slot[m] (int32, device; -1: none)."""
+        import torch
+        _device_tensor(x, "x", (torch.float32, torch.float16, torch.bfloat16), 0, self.cols)
+        m = x.shape[0]
+        _ints(slot, "slot", m)
+        _device_tensor(y, "y", (torch.float32,), m, self.rows)
+        if base is not None:
+            _device_tensor(base, "base", (torch.float32,), m, self.rows)
+        check(load().eif_hip_adapters_linear(self.h, ptr(x), _row_type(x), x.stride(0), ptr(slot), ptr(base),
+                                             0 if base is None else base.stride(0), ptr(y), y.stride(0), m, stream_ptr(stream)),
+              "eif_hip_adapters_linear")
 
 
 class BitnetModel:
