@@ -13,7 +13,8 @@
 
 // Resident: per slot A, then B, of the adapters' type, zeros beyond rank, cols and rows, each in the order in which a wave reads it:
 //   A [16 ranks][32 columns][lane][8]: lane l has rank l % 16 of the 16 and columns 8 (l / 16) .. + 7 of the 32;
-//   B [16 rows][lane][16 ranks][4]: lane l has row l % 16 of the 16 and ranks 4 (l / 16) .. + 3 of each 16.
+//   B [16 rows][32 ranks][lane][8]: lane l has row l % 16 of the 16 and ranks 4 (l / 16) .. + 3 of the first 16, then of the other 16;
+//     where the last 32 are only 16, [lane][4].
 // These are operands of the matrix instructions, and the sums of the first product (ranks 4 (l / 16) .. + 3 in lane l) those of the second.
 // And a rank (0: empty) and scale.
 struct AdapterMeta {
@@ -68,6 +69,9 @@ EIF_DEV Pack<T, 8> x_pack(const T *xr, int c, int cols)
     return p;
 }
 
+// Where a lane's part of 16 rows' B begins, and in it that of ranks 16 r .. + 15.
+EIF_DEV int b_part(int r, int rank_tiles, int lane) { return (r >> 1) * 512 + (r + 1 == rank_tiles && !(r & 1) ? lane * 4 : lane * 8 + (r & 1) * 4); }
+
 struct AdapterArgs {
     const void *x;
     const int32_t *slot;
@@ -79,6 +83,7 @@ struct AdapterArgs {
     size_t slot_bytes;
     int M, slots, rows, cols, rank_tiles, col_blocks, row_tiles;   // of the resident layout: 16 ranks, 32 columns, 16 rows
     int splits;      // workgroups that share the outputs of a row, or of a tile of rows
+    int tiles_xcd;   // tiles of rows that an XCD takes, one behind the other: rows of a prompt share an adapter, and its L2 holds it
     bool vec_y;      // base and y rows start at 16 bytes and have a multiple of four columns
 };
 
@@ -99,49 +104,75 @@ EIF_DEV void by_tiles(int n, F f)
 
 // A few rows: a workgroup of 16 waves has one row and 1024 of its outputs. It computes the row's whole A x, which workgroups of the
 // same row repeat (out of the XCD's L2, where they all run), and from it its outputs: one launch instead of two with the sums of the
-// first in memory between them.
-template <typename X, typename W, bool VEC>
+// first in memory between them. What a CU reads through its L1 bounds it (64 bytes a clock), so that x, which 16 lanes share, comes
+// from LDS. ONE: ranks up to 16, whose matrices are read before the rank is known (what lies behind it is zeros).
+template <typename X, typename W, bool VEC, bool ONE>
 __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
 {
-    __shared__ float part[16][kMaxRank];
-    __shared__ v4f v[kMaxRank / 4];
+    constexpr int R = ONE ? 16 : kMaxRank, kCols = 4096;
+    __shared__ float part[16][R];
+    __shared__ v4f v[R / 4];
+    __shared__ v4f xs[kCols / 4];   // columns of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t16 = lane & 15, q = lane >> 4;
     const int i8 = blockIdx.x / 8, row = i8 / a.splits * 8 + blockIdx.x % 8, n0 = i8 % a.splits * 1024;
     if (row >= a.M) return;
+    const X *x = static_cast<const X *>(a.x) + row * a.ldx;
+    const auto x_quad = [&](int c) {   // four columns, zeros behind the last
+        v4f r = {};
+        if constexpr (VEC) {
+            if (c < a.cols) {
+                const Pack<X, 4> p = load<4>(x + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = to_f32(p.v[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.cols) r[j] = to_f32(x[c + j]);
+        }
+        return r;
+    };
+    const v4f x0 = x_quad(tid * 4);
     const int s = slot_of(a, row), n = n0 + tid;
     const float base = a.base && n < a.rows ? a.base[row * a.ldbase + n] : 0.0f;
     float *y = a.y + row * a.ldy + n;
-    const int rank = s < 0 ? 0 : a.meta[s].rank;
-    if (rank == 0) {
+    const AdapterMeta meta = s < 0 ? AdapterMeta{} : a.meta[s];
+    if (ONE ? s < 0 : meta.rank == 0) {
         if (n < a.rows) *y = base;
         return;
     }
-    const X *x = static_cast<const X *>(a.x) + row * a.ldx;
     const W *A = reinterpret_cast<const W *>(a.data + s * a.slot_bytes);
     const W *B = A + (size_t)a.rank_tiles * a.col_blocks * 512;
-    const int tiles = (rank + 15) / 16;
+    const int tiles = ONE ? 1 : (meta.rank + 15) / 16;
     for (int r0 = 0; r0 < tiles; r0 += 4) {
-        by_tiles(min(tiles - r0, 4), [&](auto n_) {
-            constexpr int RN = decltype(n_)::value, U = RN == 4 ? 2 : 4;
+        by_tiles(ONE ? 1 : min(tiles - r0, 4), [&](auto n_) {
+            constexpr int RN = decltype(n_)::value, U = (RN == 4 ? 4 : 8) / (sizeof(W) == 4 ? 2 : 1);
             float acc[RN] = {};
-            for (int cb = wave; cb < a.col_blocks; cb += 16 * U) {
-                Pack<W, 8> w[U][RN];
-                Pack<X, 8> xv[U];
+            for (int k = 0; k < a.col_blocks; k += kCols / 32) {   // a wave has every 16th block of 32 columns
+                const int end = min(k + kCols / 32, a.col_blocks);
+                for (int cb = k + wave; cb < k + kCols / 32; cb += 16 * U) {
+                    Pack<W, 8> w[U][RN];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int b = min(cb + 16 * u, a.col_blocks - 1);
-                    xv[u] = x_pack<VEC>(x, b * 32 + q * 8, a.cols);
+                    for (int u = 0; u < U; ++u) {
 #pragma unroll
-                    for (int r = 0; r < RN; ++r)
-                        w[u][r] = load<8>(A + ((size_t)min(r0 + r, a.rank_tiles - 1) * a.col_blocks + b) * 512 + lane * 8);
-                }
+                        for (int r = 0; r < RN; ++r)
+                            w[u][r] = load<8>(A + ((size_t)min(r0 + r, a.rank_tiles - 1) * a.col_blocks + min(cb + 16 * u, end - 1)) * 512 + lane * 8);
+                    }
+                    if (cb == k + wave && (r0 == 0 || a.col_blocks > kCols / 32)) {   // the waves' loads are under way
+                        if (r0 + k > 0) __syncthreads();
+                        xs[tid] = k == 0 && r0 == 0 ? x0 : x_quad(k * 32 + tid * 4);
+                        __syncthreads();
+                    }
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (cb + 16 * u >= a.col_blocks) break;
+                    for (int u = 0; u < U; ++u) {
+                        if (cb + 16 * u < end) {
+                            const v4f lo = xs[(cb + 16 * u - k) * 8 + q * 2], hi = xs[(cb + 16 * u - k) * 8 + q * 2 + 1];
 #pragma unroll
-                    for (int r = 0; r < RN; ++r) {
+                            for (int r = 0; r < RN; ++r) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) acc[r] = fmaf(to_f32(xv[u].v[j]), to_f32(w[u][r].v[j]), acc[r]);
+                                for (int j = 0; j < 8; ++j) acc[r] = fmaf(j < 4 ? lo[j & 3] : hi[j & 3], to_f32(w[u][r].v[j]), acc[r]);
+                            }
+                        }
                     }
                 }
             }
@@ -153,25 +184,49 @@ __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
             }
         });
     }
+    // a wave has 4 tiles of 16 outputs; B's first ranks are on their way while the waves' sums meet
+    constexpr int RB = ONE ? 1 : 4;
+    const int nt0 = n0 / 16 + wave * 4;
+    Pack<W, 4> bw[4][RB];
+    const W *Bt[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        Bt[t] = B + (size_t)min(nt0 + t, a.row_tiles - 1) * a.rank_tiles * 256;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) bw[t][r] = load<4>(Bt[t] + b_part(min(r, tiles - 1), a.rank_tiles, lane));
+    }
     __syncthreads();
     if (tid < tiles * 16) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 16; ++w) sum += part[w][tid];
-        reinterpret_cast<float *>(v)[tid] = tid < rank ? sum * a.meta[s].scale : 0.0f;   // an infinite x makes NaN of the zeros beyond the rank
+        reinterpret_cast<float *>(v)[tid] = tid < meta.rank ? sum * meta.scale : 0.0f;   // an infinite x makes NaN of the zeros beyond the rank
     }
     __syncthreads();
-    // a wave has 4 tiles of 16 outputs; a lane sums its ranks, and the four lanes of an output meet in the lane whose output it is
-    const int nt0 = n0 / 16 + wave * 4;
     if (nt0 >= a.row_tiles) return;
+    if (ONE && meta.rank == 0) {   // what an empty slot holds is nothing to compute with
+        if (n < a.rows) *y = base;
+        return;
+    }
+    // a lane sums its ranks, and the four lanes of an output meet in the lane whose output it is
     float sum[4] = {};
-    for (int r = 0; r < tiles; ++r) {
-        const v4f vr = v[r * 4 + q];
+    for (int r0 = 0; r0 < tiles; r0 += RB) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const Pack<W, 4> w = load<4>(B + ((size_t)min(nt0 + t, a.row_tiles - 1) * 64 + lane) * a.rank_tiles * 4 + r * 4);
+        for (int r = 0; r < RB; ++r) {
+            if (r0 + r >= tiles) break;
+            const v4f vr = v[(r0 + r) * 4 + q];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[t] = fmaf(to_f32(w.v[j]), vr[j], sum[t]);
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[t] = fmaf(to_f32(bw[t][r].v[j]), vr[j], sum[t]);
+            }
+        }
+        if (r0 + RB < tiles) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int r = 0; r < RB; ++r) bw[t][r] = load<4>(Bt[t] + b_part(min(r0 + RB + r, tiles - 1), a.rank_tiles, lane));
+            }
         }
     }
     const bool high = lane & 32, odd = lane & 16;
@@ -213,153 +268,275 @@ EIF_DEV void planes4(v4f v, uint2 *p)
         p[i] = make_uint2(__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302));
 }
 
-// Many rows: a workgroup of 8 waves has 16 rows and a share of their outputs, and takes the adapters that its rows name one after
-// another (rows of a prompt share theirs). First V = A x of the 16 rows: the waves split the columns, and their sums meet in LDS. Then
-// B V, a tile of 16 outputs at a time, the tokens being the columns in both products. bf16 B: V as three bf16 planes on 16x16x32
-// instructions, whose products are exact, a sixteenth of the time of FP32 ones; else FP32 instructions.
-template <typename X, typename W, bool VEC>
-__global__ __launch_bounds__(512) void adapter_tile_kernel(AdapterArgs a)
+// Many rows: a workgroup of 8 waves has TT tiles of 16 rows and a share of their outputs. First V = A x of the rows, by one adapter
+// after another that they name (rows of a prompt share theirs): the waves split the columns, and their sums meet in LDS, where each
+// row keeps those of its own adapter. Then base + B V, two tiles of 16 outputs at a time, with every adapter in turn, each row taking its
+// own one's. The tokens are the columns of both products. bf16 B: V as three bf16 planes on 16x16x32 instructions, whose products are
+// exact, a sixteenth of the time of FP32 ones; else FP32 instructions. Loads run ahead: x and A two or four steps, base and B two or three.
+template <typename X, typename W, bool VEC, int TT>
+__global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(AdapterArgs a)
 {
     constexpr bool planes = std::is_same<W, __hip_bfloat16>::value;
-    __shared__ v4f part[8][4][64];
-    __shared__ v4f vs[planes ? 1 : kMaxRank / 16][64];                       // V [16 ranks][lane]
-    __shared__ uint4 vp[planes ? kMaxRank / 32 : 1][3][64];                  // [32 ranks][plane][lane]
+    constexpr int kChunk = 4;   // tiles of 16 ranks that are taken at a time
+    constexpr int DX = VEC && sizeof(X) == 2 ? 4 : 2, DW = sizeof(W) == 2 ? 2 : 1;   // steps of x and A under way: what the registers hold
+    __shared__ v4f part[8][kChunk][TT][64];
+    __shared__ v4f vs[planes ? 1 : kMaxRank / 16][TT][64];          // V [16 ranks][tile of rows][lane]
+    __shared__ uint4 vp[planes ? kMaxRank / 32 : 1][3][TT][64];     // [32 ranks][plane][tile of rows][lane]
+    __shared__ int2 step_of[TT * 16 * kMaxRank / 16 / kChunk];      // what the second product goes through: slot, first tile of ranks
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t16 = lane & 15, q = lane >> 4;
-    const int i8 = blockIdx.x / 8, tile = i8 / a.splits * 8 + blockIdx.x % 8, split = i8 % a.splits;
-    if (tile * 16 >= a.M) return;
-    const int row = min(tile * 16 + t16, a.M - 1);
-    int s = slot_of(a, row);
-    if (s >= 0 && a.meta[s].rank == 0) s = -1;
-    const bool live = tile * 16 + t16 < a.M;
-    const X *x = static_cast<const X *>(a.x) + row * a.ldx;
-    const float *base = a.base ? a.base + row * a.ldbase : nullptr;
-    float *y = a.y + row * a.ldy;
-    const int groups = (a.row_tiles + 3) / 4;   // of four tiles of outputs
-    const int from = (int)((int64_t)groups * split / a.splits), to = (int)((int64_t)groups * (split + 1) / a.splits);
+    const int i8 = blockIdx.x / 8, tile = (int)(blockIdx.x % 8) * a.tiles_xcd + i8 / a.splits, split = i8 % a.splits;
+    if (i8 / a.splits >= a.tiles_xcd || tile * (16 * TT) >= a.M) return;
+    int row[TT], s[TT];
+    bool live[TT];
+    const X *x[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const int r = (tile * TT + t) * 16 + t16;
+        live[t] = r < a.M;
+        row[t] = min(r, a.M - 1);
+        x[t] = static_cast<const X *>(a.x) + row[t] * a.ldx;
+    }
+    const int per = (a.col_blocks + 7) / 8, c0 = wave * per, c1 = min(c0 + per, a.col_blocks);
+    Pack<X, 8> xr[DX][TT];
+    const auto load_x = [&](Pack<X, 8> *p, int b) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) p[t] = x_pack<VEC>(x[t], min(b, a.col_blocks - 1) * 32 + q * 8, a.cols);
+    };
+#pragma unroll
+    for (int u = 0; u < DX; ++u) load_x(xr[u], c0 + u);
+    uint32_t left = 0;   // rows whose adapter is still to come
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        s[t] = slot_of(a, row[t]);
+        if (s[t] >= 0 && a.meta[s[t]].rank == 0) s[t] = -1;
+        left |= ((uint32_t)__ballot(live[t] && s[t] >= 0) & 0xffff) << (16 * t);
+    }
 
-    // the same in every wave: which of the 16 rows are left
-    uint32_t left = (uint32_t)__ballot(live) & 0xffff;
+    int steps = 0, most = 0;   // of the second product, and the most tiles of ranks in one; the same in every wave
     while (left) {
-        const int now = __builtin_amdgcn_readlane(s, __builtin_ctz(left));
-        const bool mine = live && s == now;
-        left &= ~(uint32_t)__ballot(mine);
-        if (now < 0 && a.base == a.y) continue;
-        const int rank = now < 0 ? 0 : a.meta[now].rank, tiles = (rank + 15) / 16;
-        const W *A = reinterpret_cast<const W *>(a.data + max(now, 0) * a.slot_bytes);
-        const W *B = A + (size_t)a.rank_tiles * a.col_blocks * 512;
-        const float scale = now < 0 ? 0.0f : a.meta[now].scale;
-        for (int r0 = 0; r0 < tiles; r0 += 4) {
-            const int rn = min(tiles - r0, 4);
+        const int first = __builtin_ctz(left);
+        int now = __builtin_amdgcn_readlane(s[0], first & 15);
+        if (TT == 2 && first >= 16) now = __builtin_amdgcn_readlane(s[TT - 1], first & 15);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) left &= ~(((uint32_t)__ballot(s[t] == now) & 0xffff) << (16 * t));
+        const int rank = a.meta[now].rank, tiles = (rank + 15) / 16;
+        const float scale = a.meta[now].scale;
+        const W *A = reinterpret_cast<const W *>(a.data + now * a.slot_bytes);
+        for (int r0 = 0; r0 < tiles; r0 += kChunk) {
+            const int rn = min(tiles - r0, kChunk);
+            if (steps > 0) {
+#pragma unroll
+                for (int u = 0; u < DX; ++u) load_x(xr[u], c0 + u);
+            }
             by_tiles(rn, [&](auto n_) {
-                constexpr int RN = decltype(n_)::value, U = RN == 4 ? 2 : 4;
-                v4f acc[RN] = {};
-                for (int cb = wave * U; cb < a.col_blocks; cb += 8 * U) {
-                    Pack<W, 8> w[U][RN];
-                    Pack<X, 8> xv[U];
+                constexpr int RN = decltype(n_)::value;
+                const W *Ar[RN];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int b = min(cb + u, a.col_blocks - 1);
-                        xv[u] = x_pack<VEC>(x, b * 32 + q * 8, a.cols);
+                for (int r = 0; r < RN; ++r) Ar[r] = A + (size_t)min(r0 + r, a.rank_tiles - 1) * a.col_blocks * 512 + lane * 8;
+                v4f acc[RN][TT] = {};
+                Pack<W, 8> w[DW][RN];
+                const auto load_w = [&](Pack<W, 8> *p, int b) {
 #pragma unroll
-                        for (int r = 0; r < RN; ++r)
-                            w[u][r] = load<8>(A + ((size_t)min(r0 + r, a.rank_tiles - 1) * a.col_blocks + b) * 512 + lane * 8);
-                    }
+                    for (int r = 0; r < RN; ++r) p[r] = load<8>(Ar[r] + (size_t)min(b, a.col_blocks - 1) * 512);
+                };
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (cb + u >= a.col_blocks) break;
+                for (int u = 0; u < DW; ++u) load_w(w[u], c0 + u);
+                for (int cb = c0; cb < c1; cb += DX) {
 #pragma unroll
-                        for (int r = 0; r < RN; ++r) acc[r] = product32(w[u][r], xv[u], acc[r]);
+                    for (int u = 0; u < DX; ++u) {
+                        if (cb + u < c1) {
+#pragma unroll
+                            for (int r = 0; r < RN; ++r) {
+#pragma unroll
+                                for (int t = 0; t < TT; ++t) acc[r][t] = product32(w[u % DW][r], xr[u][t], acc[r][t]);
+                            }
+                            load_x(xr[u], cb + u + DX);
+                            load_w(w[u % DW], cb + u + DW);
+                        }
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < RN; ++r) part[wave][r][lane] = acc[r];
+                for (int r = 0; r < RN; ++r) {
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) part[wave][r][t][lane] = acc[r][t];
+                }
             });
+            if (tid == 0) step_of[steps] = make_int2(now, r0);
             __syncthreads();
-            if (wave < 4) {
+            if (wave < kChunk * TT) {   // a wave sums a tile of ranks of a tile of rows
+                const int r = wave / TT, t = wave % TT;
+                const bool mine = (TT == 1 || t == 0 ? s[0] : s[TT - 1]) == now;
                 v4f sum = {};
-                if (wave < rn) {
+                if (r < rn) {
 #pragma unroll
-                    for (int w = 0; w < 8; ++w) sum += part[w][wave][lane];
+                    for (int w = 0; w < 8; ++w) sum += part[w][r][t][lane];
+                    // an infinite x makes NaN of the zeros beyond the rank
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[j] = (r0 + wave) * 16 + q * 4 + j < rank ? sum[j] * scale : 0.0f;
+                    for (int j = 0; j < 4; ++j) sum[j] = (r0 + r) * 16 + q * 4 + j < rank ? sum[j] * scale : 0.0f;
                 }
                 if constexpr (planes) {
                     uint2 p[3];
                     planes4(sum, p);
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) reinterpret_cast<uint2 *>(&vp[(r0 + wave) / 2][i][lane])[wave & 1] = p[i];
-                } else {
-                    vs[r0 + wave][lane] = sum;
+                    for (int i = 0; i < 3; ++i)
+                        if (mine) reinterpret_cast<uint2 *>(&vp[(r0 + r) / 2][i][t][lane])[r & 1] = p[i];
+                } else if (mine) {
+                    vs[r0 + r][t][lane] = sum;
                 }
             }
             __syncthreads();
+            ++steps;
+            most = max(most, rn);
         }
-        const int pairs = (tiles + 1) / 2;
-        for (int g = from + wave; g < to; g += 8) {
-            const int nt0 = g * 4, n0 = nt0 * 16 + q * 4;
-            v4f add[4], acc[4] = {};
-            const W *Bl[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int n = n0 + t * 16;
-                add[t] = v4f{};
-                if (mine && base) {
-                    if (a.vec_y) {
-                        if (n < a.rows) add[t] = *reinterpret_cast<const v4f *>(base + n);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (n + j < a.rows) add[t][j] = base[n + j];
-                    }
-                }
-                Bl[t] = B + ((size_t)min(nt0 + t, a.row_tiles - 1) * 64 + lane) * a.rank_tiles * 4;
-            }
-            if constexpr (planes) {
-                for (int p = 0; p < pairs; ++p) {
-                    uint4 w[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint2 *b = reinterpret_cast<const uint2 *>(Bl[t] + p * 8);
-                        const uint2 lo = b[0], hi = p * 2 + 1 < tiles ? b[1] : make_uint2(0, 0);
-                        w[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                    }
-#pragma unroll
-                    for (int i = 2; i >= 0; --i) {
-                        const uint4 v = vp[p][i][lane];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w[t]), __builtin_bit_cast(v8bf, v), acc[t], 0, 0, 0);
-                    }
-                }
+    }
+
+    const bool in_place = a.base == a.y;
+    if (steps == 0 && in_place) return;
+    const int groups = (a.row_tiles + 1) / 2;   // of two tiles of outputs
+    const int from = (int)((int64_t)groups * split / a.splits), to = (int)((int64_t)groups * (split + 1) / a.splits);
+    // rows often lie a power of two apart: tiles of rows begin at different outputs, so as not to meet in the same memory channels
+    const int turn = to > from ? (int)((unsigned)(tile * TT) * 5u % (unsigned)(to - from)) : 0;
+    const auto tile_of = [&](int g) { return 2 * (g + turn < to ? g + turn : g + turn - (to - from)); };
+    const auto load_base = [&](int t, int n) {
+        v4f v = {};
+        if (a.base) {
+            const float *base = a.base + row[t] * a.ldbase;
+            if (a.vec_y) {
+                v = *reinterpret_cast<const v4f *>(base + min(n, a.rows - 4));
             } else {
-                for (int r = 0; r < tiles; ++r) {
-                    const v4f v = vs[r][lane];
-                    Pack<W, 4> w[4];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) w[t] = load<4>(Bl[t] + r * 4);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w[t].v[j]), v[j], acc[t], 0, 0, 0);
-                    }
-                }
+                for (int j = 0; j < 4; ++j) v[j] = base[min(n + j, a.rows - 1)];
             }
-            if (!mine) continue;
+        }
+        return v;
+    };
+    const auto store_y = [&](int t, int n, v4f v) {
+        if (!live[t] || (s[t] < 0 && in_place)) return;
+        float *y = a.y + row[t] * a.ldy;
+        if (a.vec_y) {
+            if (n < a.rows) *reinterpret_cast<v4f *>(y + n) = v;
+        } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int n = n0 + t * 16;
-                const v4f o = add[t] + acc[t];
-                if (a.vec_y) {
-                    if (n < a.rows) *reinterpret_cast<v4f *>(y + n) = o;
+            for (int j = 0; j < 4; ++j)
+                if (n + j < a.rows) y[n + j] = v[j];
+        }
+    };
+    if (steps == 0) {
+        for (int g = from + wave; g < to; g += 8) {
+            const int n = tile_of(g) * 16 + q * 4;
+            v4f v[TT][2];
+#pragma unroll
+            for (int i = 0; i < 2 * TT; ++i) v[i / 2][i % 2] = load_base(i / 2, n + i % 2 * 16);
+#pragma unroll
+            for (int i = 0; i < 2 * TT; ++i) store_y(i / 2, n + i % 2 * 16, v[i / 2][i % 2]);
+        }
+        return;
+    }
+    by_tiles(most, [&](auto n_) {
+        constexpr int RT = decltype(n_)::value, D = sizeof(W) == 2 ? 3 : 2;
+        struct Ahead {
+            v4f add[TT][2];
+            Pack<W, 4> w[2][RT];
+        } ahead[D];
+        int gl = from + wave, sl = 0;   // the group and step to load next
+        const auto load_next = [&](Ahead &h) {
+            if (gl >= to) return;
+            const int nt = tile_of(gl);
+            const int2 st = step_of[sl];
+            const int slot = __builtin_amdgcn_readfirstlane(st.x), r0 = __builtin_amdgcn_readfirstlane(st.y);
+            const W *B = reinterpret_cast<const W *>(a.data + slot * a.slot_bytes) + (size_t)a.rank_tiles * a.col_blocks * 512;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (sl == 0) {
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) h.add[t][i] = load_base(t, (nt + i) * 16 + q * 4);
+                }
+                const W *b = B + (size_t)min(nt + i, a.row_tiles - 1) * a.rank_tiles * 256;
+                if constexpr (RT == 1) {
+                    h.w[i][0] = load<4>(b + b_part(r0, a.rank_tiles, lane));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (n + j < a.rows) y[n + j] = o[j];
+                    for (int r = 0; r < RT; r += 2) {
+                        if (r0 + r + 1 < a.rank_tiles) {   // both of the 32
+                            const Pack<W, 8> p = load<8>(b + (r0 + r) * 256 + lane * 8);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) h.w[i][r].v[j] = p.v[j], h.w[i][r + 1].v[j] = p.v[4 + j];
+                        } else {
+                            h.w[i][r] = h.w[i][r + 1] = load<4>(b + b_part(min(r0 + r, a.rank_tiles - 1), a.rank_tiles, lane));
+                        }
+                    }
+                }
+            }
+            if (++sl == steps) {
+                sl = 0;
+                gl += 8;
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d) load_next(ahead[d]);
+        int g = from + wave, at = 0;
+        v4f sum[TT][2];
+        while (g < to) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (g < to) {
+                    Ahead &h = ahead[d];
+                    const int2 st = step_of[at];
+                    const int r0 = __builtin_amdgcn_readfirstlane(st.y);
+                    v4f acc[TT][2] = {};
+                    if constexpr (planes) {
+#pragma unroll
+                        for (int p = 0; p < (RT + 1) / 2; ++p) {
+                            v8bf w[2];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint2 lo = __builtin_bit_cast(uint2, h.w[i][2 * p]);
+                                const uint2 hi = RT > 1 ? __builtin_bit_cast(uint2, h.w[i][RT > 1 ? 2 * p + 1 : 0]) : make_uint2(0, 0);
+                                w[i] = __builtin_bit_cast(v8bf, make_uint4(lo.x, lo.y, hi.x, hi.y));
+                            }
+#pragma unroll
+                            for (int i = 2; i >= 0; --i) {
+#pragma unroll
+                                for (int t = 0; t < TT; ++t) {
+                                    const v8bf v = __builtin_bit_cast(v8bf, vp[r0 / 2 + p][i][t][lane]);
+                                    acc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[0], v, acc[t][0], 0, 0, 0);
+                                    acc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[1], v, acc[t][1], 0, 0, 0);
+                                }
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+#pragma unroll
+                            for (int t = 0; t < TT; ++t) {
+                                const v4f v = vs[r0 + r][t][lane];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    acc[t][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(h.w[0][r].v[j]), v[j], acc[t][0], 0, 0, 0);
+                                    acc[t][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(h.w[1][r].v[j]), v[j], acc[t][1], 0, 0, 0);
+                                }
+                            }
+                        }
+                    }
+                    const int n = tile_of(g) * 16 + q * 4;
+#pragma unroll
+                    for (int i = 0; i < 2 * TT; ++i) {
+                        v4f &o = sum[i / 2][i % 2];
+                        const v4f &p = acc[i / 2][i % 2];
+                        if (at == 0) o = h.add[i / 2][i % 2];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[j] = s[i / 2] == st.x ? o[j] + p[j] : o[j];
+                        if (at + 1 == steps) store_y(i / 2, n + i % 2 * 16, o);
+                    }
+                    load_next(h);
+                    if (++at == steps) {
+                        at = 0;
+                        g += 8;
+                    }
                 }
             }
         }
-        __syncthreads();   // V is the next adapter's
-    }
+    });
 }
 
 // An adapter into its place, zeros around it, and its rank and scale.
@@ -375,15 +552,33 @@ __global__ __launch_bounds__(256) void adapter_set_kernel(const W *A, int64_t ld
         const int lane = (int)(i / 8) & 63, r = (int)(i / 512 / col_blocks) * 16 + lane % 16, c = (int)(i / 512 % col_blocks) * 32 + lane / 16 * 8 + (int)(i & 7);
         if (r < rank && c < cols) v = A[r * lda + c];
     } else {
-        const int64_t k = i - na, of_lane = k / (rank_tiles * 4);
-        const int at = (int)(k - of_lane * (rank_tiles * 4)), lane = (int)of_lane & 63;
-        const int n = (int)(of_lane / 64) * 16 + lane % 16, r = at / 4 * 16 + lane / 16 * 4 + at % 4;
+        const int64_t k = i - na, nt = k / (rank_tiles * 256);
+        const int at = (int)(k - nt * (rank_tiles * 256)), p = at / 512, in = at % 512;
+        const bool half = 2 * p + 1 == rank_tiles;   // 16 ranks alone
+        const int lane = half ? in / 4 : in / 8, n = (int)nt * 16 + lane % 16, r = p * 32 + (half ? 0 : in % 8 / 4 * 16) + lane / 16 * 4 + in % 4;
         if (n < rows && r < rank) v = B[n * ldb + r];
     }
     to[i] = v;
 }
 
 // ---- launches ----
+
+template <typename X, typename W, bool VEC, int TT>
+int launch_tiles_as(AdapterArgs a, int workgroups, hipStream_t st)
+{
+    const int tiles = eif_ceil_div(a.M, 16 * TT);
+    a.splits = std::max(1, std::min(eif_ceil_div(a.rows, 128), workgroups / tiles));
+    a.tiles_xcd = eif_ceil_div(tiles, 8);
+    adapter_tile_kernel<X, W, VEC, TT><<<(unsigned)(a.tiles_xcd * 8 * a.splits), 512, 0, st>>>(a);
+    EIF_HIP_LAUNCHED();
+    return EIF_HIP_OK;
+}
+
+template <typename X, typename W, bool VEC>
+int launch_tiles(const AdapterArgs &a, hipStream_t st)
+{
+    return a.M >= 4096 ? launch_tiles_as<X, W, VEC, 2>(a, 256, st) : launch_tiles_as<X, W, VEC, 1>(a, 512, st);
+}
 
 template <typename X, typename W>
 int launch_adapters_as(AdapterArgs a, hipStream_t st)
@@ -392,18 +587,12 @@ int launch_adapters_as(AdapterArgs a, hipStream_t st)
     if (a.M <= 64) {
         a.splits = eif_ceil_div(a.rows, 1024);
         const unsigned blocks = (unsigned)(eif_ceil_div(a.M, 8) * 8 * a.splits);
-        if (vec)
-            adapter_rows_kernel<X, W, true><<<blocks, 1024, 0, st>>>(a);
+        if (a.rank_tiles == 1)
+            vec ? adapter_rows_kernel<X, W, true, true><<<blocks, 1024, 0, st>>>(a) : adapter_rows_kernel<X, W, false, true><<<blocks, 1024, 0, st>>>(a);
         else
-            adapter_rows_kernel<X, W, false><<<blocks, 1024, 0, st>>>(a);
+            vec ? adapter_rows_kernel<X, W, true, false><<<blocks, 1024, 0, st>>>(a) : adapter_rows_kernel<X, W, false, false><<<blocks, 1024, 0, st>>>(a);
     } else {
-        const int tiles = eif_ceil_div(a.M, 16);
-        a.splits = std::max(1, std::min(eif_ceil_div(a.rows, 128), 512 / tiles));
-        const unsigned blocks = (unsigned)(eif_ceil_div(tiles, 8) * 8 * a.splits);
-        if (vec)
-            adapter_tile_kernel<X, W, true><<<blocks, 512, 0, st>>>(a);
-        else
-            adapter_tile_kernel<X, W, false><<<blocks, 512, 0, st>>>(a);
+        return vec ? launch_tiles<X, W, true>(a, st) : launch_tiles<X, W, false>(a, st);
     }
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
