@@ -93,7 +93,7 @@ EIF_DEV int slot_of(const AdapterArgs &a, int row)
     return (unsigned)s < (unsigned)a.slots ? s : -1;
 }
 
-// f with the count of 16-rank tiles that are taken at a time: 1, 2 or 4 (of 3: the fourth is computed of what lies there and not used).
+// f with the count of 16-rank tiles that are taken at a time: 1, 2 or 4 (of 3, the fourth is computed of what lies there and not used).
 template <typename F>
 EIF_DEV void by_tiles(int n, F f)
 {
@@ -268,21 +268,24 @@ EIF_DEV void planes4(v4f v, uint2 *p)
         p[i] = make_uint2(__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302));
 }
 
-// Many rows: a workgroup of 8 waves has TT tiles of 16 rows and a share of their outputs. First V = A x of the rows, by one adapter
-// after another that they name (rows of a prompt share theirs): the waves split the columns, and their sums meet in LDS, where each
-// row keeps those of its own adapter. Then base + B V, two tiles of 16 outputs at a time, with every adapter in turn, each row taking its
-// own one's. The tokens are the columns of both products. bf16 B: V as three bf16 planes on 16x16x32 instructions, whose products are
-// exact, a sixteenth of the time of FP32 ones; else FP32 instructions. Loads run ahead: x and A two or four steps, base and B two or three.
+// Many rows: a workgroup of 8 waves has TT tiles of 16 rows and a share of their outputs. First V = A x of the rows, for all the
+// adapters that they name (rows of a prompt share theirs), 4 tiles of 16 ranks at a time: the waves split the columns, and their
+// sums meet in LDS, where each row keeps those of its own adapter. Then base + B V, two tiles of 16 outputs at a time, with every adapter in
+// turn, each row taking its own one's. The tokens are the columns of both products. bf16 B: V as three bf16 planes on 16x16x32
+// instructions, whose products are exact, a sixteenth of the time of FP32 ones; else FP32 instructions. Loads run ahead: x and A two or
+// four steps, base and B two or three.
 template <typename X, typename W, bool VEC, int TT>
 __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(AdapterArgs a)
 {
     constexpr bool planes = std::is_same<W, __hip_bfloat16>::value;
-    constexpr int kChunk = 4;   // tiles of 16 ranks that are taken at a time
-    constexpr int DX = VEC && sizeof(X) == 2 ? 4 : 2, DW = sizeof(W) == 2 ? 2 : 1;   // steps of x and A under way: what the registers hold
+    constexpr int DW = VEC && sizeof(W) == 2 ? 2 : 1;                   // and of A: DX is a multiple of it
+    constexpr int kChunk = 4;   // tiles of 16 ranks that a pass over x takes, and a step of the second product
+    constexpr int DX = !VEC ? 1 : sizeof(X) == 2 && planes ? 4 : 2;   // steps of x under way, as many as the registers hold
     __shared__ v4f part[8][kChunk][TT][64];
     __shared__ v4f vs[planes ? 1 : kMaxRank / 16][TT][64];          // V [16 ranks][tile of rows][lane]
     __shared__ uint4 vp[planes ? kMaxRank / 32 : 1][3][TT][64];     // [32 ranks][plane][tile of rows][lane]
-    __shared__ int2 step_of[TT * 16 * kMaxRank / 16 / kChunk];      // what the second product goes through: slot, first tile of ranks
+    __shared__ int2 tile_at[TT * 16 * kMaxRank / 16];               // what the first product goes through: slot, tile of ranks
+    __shared__ int2 step_at[TT * 16 * kMaxRank / 16 / kChunk];      // and the second: slot, first tile of ranks
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t16 = lane & 15, q = lane >> 4;
     const int i8 = blockIdx.x / 8, tile = (int)(blockIdx.x % 8) * a.tiles_xcd + i8 / a.splits, split = i8 % a.splits;
     if (i8 / a.splits >= a.tiles_xcd || tile * (16 * TT) >= a.M) return;
@@ -312,82 +315,93 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
         left |= ((uint32_t)__ballot(live[t] && s[t] >= 0) & 0xffff) << (16 * t);
     }
 
-    int steps = 0, most = 0;   // of the second product, and the most tiles of ranks in one; the same in every wave
+    int all = 0, steps = 0, most = 0;   // tiles of ranks, steps of the second product, the most tiles in one; the same in every wave
     while (left) {
         const int first = __builtin_ctz(left);
         int now = __builtin_amdgcn_readlane(s[0], first & 15);
         if (TT == 2 && first >= 16) now = __builtin_amdgcn_readlane(s[TT - 1], first & 15);
 #pragma unroll
         for (int t = 0; t < TT; ++t) left &= ~(((uint32_t)__ballot(s[t] == now) & 0xffff) << (16 * t));
-        const int rank = a.meta[now].rank, tiles = (rank + 15) / 16;
-        const float scale = a.meta[now].scale;
-        const W *A = reinterpret_cast<const W *>(a.data + now * a.slot_bytes);
-        for (int r0 = 0; r0 < tiles; r0 += kChunk) {
-            const int rn = min(tiles - r0, kChunk);
-            if (steps > 0) {
+        const int tiles = (a.meta[now].rank + 15) / 16;
+        for (int r = 0; r < tiles; r += kChunk, ++steps) {
+            if (tid < min(tiles - r, kChunk)) tile_at[all + r + tid] = make_int2(now, r + tid);
+            if (tid == 0) step_at[steps] = make_int2(now, r);
+        }
+        all += tiles;
+        most = max(most, min(tiles, kChunk));
+    }
+    __syncthreads();
+    for (int e0 = 0; e0 < all; e0 += kChunk) {
+        if (e0 > 0) {
 #pragma unroll
-                for (int u = 0; u < DX; ++u) load_x(xr[u], c0 + u);
+            for (int u = 0; u < DX; ++u) load_x(xr[u], c0 + u);
+        }
+        by_tiles(min(all - e0, kChunk), [&](auto n_) {
+            constexpr int RN = decltype(n_)::value;
+            const W *Ar[RN];
+#pragma unroll
+            for (int r = 0; r < RN; ++r) {
+                const int2 e = tile_at[min(e0 + r, all - 1)];
+                const int slot = __builtin_amdgcn_readfirstlane(e.x), rt = __builtin_amdgcn_readfirstlane(e.y);
+                Ar[r] = reinterpret_cast<const W *>(a.data + slot * a.slot_bytes) + (size_t)rt * a.col_blocks * 512;
             }
-            by_tiles(rn, [&](auto n_) {
-                constexpr int RN = decltype(n_)::value;
-                const W *Ar[RN];
+            v4f acc[RN][TT] = {};
+            Pack<W, 8> w[DW][RN];
+            const auto load_w = [&](Pack<W, 8> *p, int b) {
 #pragma unroll
-                for (int r = 0; r < RN; ++r) Ar[r] = A + (size_t)min(r0 + r, a.rank_tiles - 1) * a.col_blocks * 512 + lane * 8;
-                v4f acc[RN][TT] = {};
-                Pack<W, 8> w[DW][RN];
-                const auto load_w = [&](Pack<W, 8> *p, int b) {
+                for (int r = 0; r < RN; ++r) p[r] = load<8>(Ar[r] + (size_t)min(b, a.col_blocks - 1) * 512 + lane * 8);
+            };
 #pragma unroll
-                    for (int r = 0; r < RN; ++r) p[r] = load<8>(Ar[r] + (size_t)min(b, a.col_blocks - 1) * 512);
-                };
+            for (int u = 0; u < DW; ++u) load_w(w[u], c0 + u);
+            for (int cb = c0; cb < c1; cb += DX) {
 #pragma unroll
-                for (int u = 0; u < DW; ++u) load_w(w[u], c0 + u);
-                for (int cb = c0; cb < c1; cb += DX) {
+                for (int u = 0; u < DX; ++u) {
+                    if (cb + u < c1) {
 #pragma unroll
-                    for (int u = 0; u < DX; ++u) {
-                        if (cb + u < c1) {
+                        for (int r = 0; r < RN; ++r) {
 #pragma unroll
-                            for (int r = 0; r < RN; ++r) {
-#pragma unroll
-                                for (int t = 0; t < TT; ++t) acc[r][t] = product32(w[u % DW][r], xr[u][t], acc[r][t]);
-                            }
-                            load_x(xr[u], cb + u + DX);
-                            load_w(w[u % DW], cb + u + DW);
+                            for (int t = 0; t < TT; ++t) acc[r][t] = product32(w[u % DW][r], xr[u][t], acc[r][t]);
                         }
+                        load_x(xr[u], cb + u + DX);
+                        load_w(w[u % DW], cb + u + DW);
                     }
                 }
-#pragma unroll
-                for (int r = 0; r < RN; ++r) {
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) part[wave][r][t][lane] = acc[r][t];
-                }
-            });
-            if (tid == 0) step_of[steps] = make_int2(now, r0);
-            __syncthreads();
-            if (wave < kChunk * TT) {   // a wave sums a tile of ranks of a tile of rows
-                const int r = wave / TT, t = wave % TT;
-                const bool mine = (TT == 1 || t == 0 ? s[0] : s[TT - 1]) == now;
-                v4f sum = {};
-                if (r < rn) {
-#pragma unroll
-                    for (int w = 0; w < 8; ++w) sum += part[w][r][t][lane];
-                    // an infinite x makes NaN of the zeros beyond the rank
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[j] = (r0 + r) * 16 + q * 4 + j < rank ? sum[j] * scale : 0.0f;
-                }
-                if constexpr (planes) {
-                    uint2 p[3];
-                    planes4(sum, p);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (mine) reinterpret_cast<uint2 *>(&vp[(r0 + r) / 2][i][t][lane])[r & 1] = p[i];
-                } else if (mine) {
-                    vs[r0 + r][t][lane] = sum;
-                }
             }
-            __syncthreads();
-            ++steps;
-            most = max(most, rn);
+#pragma unroll
+            for (int r = 0; r < RN; ++r) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) part[wave][r][t][lane] = acc[r][t];
+            }
+        });
+        __syncthreads();
+        const int r = wave / TT, t = wave % TT, e = e0 + r;   // a wave sums a tile of ranks of a tile of rows
+        if (r < kChunk && e < all) {
+            const int2 at = tile_at[e];
+            const int slot = __builtin_amdgcn_readfirstlane(at.x), rt = __builtin_amdgcn_readfirstlane(at.y);
+            const AdapterMeta meta = a.meta[slot];
+            v4f sum = part[0][r][t][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) sum += part[w][r][t][lane];
+            // an infinite x makes NaN of the zeros beyond the rank
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] = rt * 16 + q * 4 + j < meta.rank ? sum[j] * meta.scale : 0.0f;
+            if ((TT == 1 || t == 0 ? s[0] : s[TT - 1]) == slot) {
+                const auto put = [&](int i, v4f v) {
+                    if constexpr (planes) {
+                        uint2 p[3];
+                        planes4(v, p);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) reinterpret_cast<uint2 *>(&vp[i / 2][k][t][lane])[i & 1] = p[k];
+                    } else {
+                        vs[i][t][lane] = v;
+                    }
+                };
+                put(rt, sum);
+                if ((rt + 1) * 16 >= meta.rank)   // zeros up to the end of the step
+                    for (int i = rt + 1; i % kChunk != 0; ++i) put(i, v4f{});
+            }
         }
+        __syncthreads();
     }
 
     const bool in_place = a.base == a.y;
@@ -433,7 +447,7 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
         return;
     }
     by_tiles(most, [&](auto n_) {
-        constexpr int RT = decltype(n_)::value, D = sizeof(W) == 2 ? 3 : 2;
+        constexpr int RT = decltype(n_)::value, D = planes ? 3 : 2;
         struct Ahead {
             v4f add[TT][2];
             Pack<W, 4> w[2][RT];
@@ -442,7 +456,7 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
         const auto load_next = [&](Ahead &h) {
             if (gl >= to) return;
             const int nt = tile_of(gl);
-            const int2 st = step_of[sl];
+            const int2 st = step_at[sl];
             const int slot = __builtin_amdgcn_readfirstlane(st.x), r0 = __builtin_amdgcn_readfirstlane(st.y);
             const W *B = reinterpret_cast<const W *>(a.data + slot * a.slot_bytes) + (size_t)a.rank_tiles * a.col_blocks * 512;
 #pragma unroll
@@ -481,7 +495,7 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
             for (int d = 0; d < D; ++d) {
                 if (g < to) {
                     Ahead &h = ahead[d];
-                    const int2 st = step_of[at];
+                    const int2 st = step_at[at];
                     const int r0 = __builtin_amdgcn_readfirstlane(st.y);
                     v4f acc[TT][2] = {};
                     if constexpr (planes) {
