@@ -39,34 +39,56 @@ struct RouteArgs {
     float scale;
 };
 
+// The value of lane l ^ LX.
 template <int LX>
-EIF_DEV double xlane_d(double v)
+EIF_DEV uint32_t xlane_u(uint32_t v)
 {
-    const float lo = xlane<LX>(__int_as_float(__double2loint(v))), hi = xlane<LX>(__int_as_float(__double2hiint(v)));
-    return __hiloint2double(__float_as_int(hi), __float_as_int(lo));
+    if constexpr (LX <= 8) {
+        return __float_as_uint(xlane<LX>(__uint_as_float(v)));
+    } else {   // the swap of half waves, or of rows of 16, leaves both values in both halves
+        const auto r = LX == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & LX) ? r[0] : r[1];
+    }
 }
 template <int LX>
-EIF_DEV float xlane_of(float v) { return xlane<LX>(v); }
+EIF_DEV float xlane_of(float v) { return __uint_as_float(xlane_u<LX>(__float_as_uint(v))); }
 template <int LX>
-EIF_DEV double xlane_of(double v) { return xlane_d<LX>(v); }
+EIF_DEV double xlane_of(double v)
+{
+    return __hiloint2double((int)xlane_u<LX>((uint32_t)__double2hiint(v)), (int)xlane_u<LX>((uint32_t)__double2loint(v)));
+}
+// The value of another lane of the row of 16, N lanes on around it.
+template <int N>
+EIF_DEV float row_turn(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false)); }
+template <int N>
+EIF_DEV double row_turn(double v)
+{
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), 0x120 + N, 0xf, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), 0x120 + N, 0xf, 0xf, false));
+}
+
+// f of the integers FIRST .. LAST as types.
+template <int FIRST, int LAST, typename F>
+EIF_DEV void for_each(F f)
+{
+    if constexpr (FIRST <= LAST) {
+        f(std::integral_constant<int, FIRST>{});
+        for_each<FIRST + 1, LAST>(f);
+    }
+}
 
 // f over the lanes l ^ 1, ^ 2, .. of a group of LPT lanes.
 template <int LPT, typename F>
 EIF_DEV void butterfly(F f)
 {
-    f(std::integral_constant<int, 1>{});
-    f(std::integral_constant<int, 2>{});
-    f(std::integral_constant<int, 4>{});
-    f(std::integral_constant<int, 8>{});
-    if constexpr (LPT == 64) {
-        f(std::integral_constant<int, 16>{});
-        f(std::integral_constant<int, 32>{});
-    }
+    for_each<0, LPT == 64 ? 5 : 3>([&](auto i) { f(std::integral_constant<int, 1 << decltype(i)::value>{}); });
 }
+template <typename V>
+EIF_DEV V larger(V a, V b) { return a > b ? a : b; }   // of numbers: nothing here is a NaN
 template <int LPT, typename V>
 EIF_DEV V lanes_max(V v)
 {
-    butterfly<LPT>([&](auto x) { v = fmax(v, xlane_of<decltype(x)::value>(v)); });
+    butterfly<LPT>([&](auto x) { v = larger(v, xlane_of<decltype(x)::value>(v)); });
     return v;
 }
 template <int LPT, typename V>
@@ -76,104 +98,175 @@ EIF_DEV V lanes_sum(V v)
     return v;
 }
 
-EIF_DEV float logit_at(const RouteArgs &a, int64_t i)
+// e^x for x <= 709.7 to about an ulp: x = n ln 2 + r with ln 2 in two parts (Cody and Waite), e^r by its Taylor series up to r^13 / 13!,
+// which |r| <= ln 2 / 2 leaves off by 5e-18. The library's function takes care of more and takes twice as long.
+EIF_DEV double exp64(double x)
 {
-    const float l = a.type == EIF_HIP_F32   ? static_cast<const float *>(a.logits)[i]
-                    : a.type == EIF_HIP_F16 ? __half2float(static_cast<const __half *>(a.logits)[i])
-                                            : __bfloat162float(static_cast<const __hip_bfloat16 *>(a.logits)[i]);
+    x = larger(x, -760.0);   // 0 as well, and n fits
+    const double n = rint(x * 1.4426950408889634);
+    double r = fma(n, -0x1.62e42fefa3800p-1, x);   // 41 bits of ln 2, so that n times it is exact
+    r = fma(n, -0x1.ef35793c76730p-45, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
+
+// 1 / d for 1 <= d < 2^1023: the instruction's 2^-26 or so and two Newton steps, each fused, so that the last rounds what it should.
+EIF_DEV double reciprocal(double d)
+{
+    double q = __builtin_amdgcn_rcp(d);
+    q = fma(fma(-d, q, 1.0), q, q);
+    return fma(fma(-d, q, 1.0), q, q);
+}
+
+// 1 / (1 + e^-l): 0 from where e^-l leaves the range of 64 bits.
+EIF_DEV double sigmoid64(double l)
+{
+    const double s = reciprocal(1.0 + exp64(-larger(l, -709.7)));
+    return l < -709.7 ? 0.0 : s;
+}
+
+template <typename T>
+EIF_DEV float logit_of(T v)
+{
+    const float l = (float)v;
     return l > -INFINITY ? fminf(l, 3.402823466e+38f) : -INFINITY;   // NaN and -inf: shut out
+}
+// Logits i LPT + sub of a row, i < VPL.
+template <int LPT, int VPL, typename T>
+EIF_DEV void load_logits(const T *row, int sub, int experts, float *l)
+{
+    T v[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] = row[min(i * LPT + sub, experts - 1)];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) l[i] = i * LPT + sub < experts ? logit_of(v[i]) : -INFINITY;
+}
+
+// Candidates of a token that LDS holds: three a lane, or one.
+constexpr int route_room(int lpt) { return lpt == 16 ? 48 : 64; }
+
+// LDS of a token, in KEYs: what the experts and groups are worth, later the candidates; and the lanes' largest.
+template <typename KEY, int LPT>
+__host__ __device__ constexpr int route_lds(int experts, int groups)
+{
+    const int kRoom = LPT == 16 ? 48 : 64;
+    const int both = 2 * kRoom * (int)sizeof(float) / (int)sizeof(KEY) + kRoom;   // a KEY, an index and a logit each
+    const int worth = groups > 1 ? experts + groups : 0;
+    return (both > worth ? both : worth) + (LPT == 64 ? 64 : 0);
 }
 
 // LPT lanes a token, lane `sub` of them has experts sub, sub + LPT, .. (VPL of them). KEY is what experts are compared by: their
 // logits (float), or score plus bias (double; experts of equal scores in 32 bits can differ in 64, and which of them is chosen
-// changes the token's result by a whole expert). The choice takes the largest top_k times over: each lane's best, the best of the lanes.
+// changes the token's result by a whole expert).
+//   The choice: the top-th largest of the lanes' largest is at most the top-th largest of all, so that the experts at or above it hold the
+// chosen ones, and are few more. They go to LDS, and each counts those that come before it. Where LDS has no room for them (many
+// equals), the largest is taken top times over.
 template <typename KEY, int LPT, int VPL>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
+EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, KEY *lds)
 {
-    extern __shared__ double lds[];
-    constexpr int per_wave = 64 / LPT;
     constexpr bool wide = sizeof(KEY) == 8;
+    constexpr int kRoom = route_room(LPT);
     const KEY none = -INFINITY;
-    const int lane = threadIdx.x & 63, sub = lane % LPT, wave = threadIdx.x >> 6;
-    const int mine = wave * per_wave + lane / LPT;   // of the workgroup's tokens
-    const int64_t token = (int64_t)blockIdx.x * (blockDim.x / LPT) + mine;
-    const bool live = token < a.tokens;
-    const int64_t row = (live ? token : a.tokens - 1) * a.ldl;
+    const int sub = lane % LPT;
+    const int64_t row = token * a.ldl;
 
+    float l[VPL];
     KEY by[VPL];
-    float m = 0.0f, z = 0.0f;   // softmax: largest logit, sum of e^(l - m)
-    double md = 0.0, zd = 0.0;
-    {
-        float l[VPL];
+    if (a.type == EIF_HIP_F32) load_logits<LPT, VPL>(static_cast<const float *>(a.logits) + row, sub, a.experts, l);
+    else if (a.type == EIF_HIP_F16) load_logits<LPT, VPL>(static_cast<const __half *>(a.logits) + row, sub, a.experts, l);
+    else load_logits<LPT, VPL>(static_cast<const __hip_bfloat16 *>(a.logits) + row, sub, a.experts, l);
+    double md = 0.0, zd = 1.0;   // softmax: largest logit, sum of e^(l - m)
+    if (a.score == EIF_HIP_SCORE_SOFTMAX && (wide || !a.renormalise)) {
+        float m = l[0];
+#pragma unroll
+        for (int i = 1; i < VPL; ++i) m = larger(m, l[i]);
+        m = lanes_max<LPT>(m);
+        if (m == -INFINITY) m = 0.0f;
+        md = m;
+        if constexpr (!wide) {
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) z += expf(l[i] - m);
+            zd = lanes_sum<LPT>(z);
+        }
+    }
+    if constexpr (wide) {
+        double p[VPL];
+        if (a.score == EIF_HIP_SCORE_SOFTMAX) {
+            zd = 0.0;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                p[i] = l[i] > -INFINITY ? exp64((double)l[i] - md) : 0.0;
+                zd += p[i];
+            }
+            zd = lanes_sum<LPT>(zd);
+            const double inverse = 1.0 / zd;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) p[i] *= inverse;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) p[i] = sigmoid64(l[i]);
+        }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int e = i * LPT + sub;
-            l[i] = e < a.experts ? logit_at(a, row + e) : -INFINITY;
+            const double b = a.bias && e < a.experts ? (double)a.bias[e] : 0.0;
+            const bool open = l[i] > -INFINITY && b > -INFINITY;
+            p[i] = open ? p[i] + b : none;
+            by[i] = !open ? none : a.bias ? p[i] : (double)l[i];
+            if (a.groups > 1 && e < a.experts) lds[e] = p[i];
         }
-        if (a.score == EIF_HIP_SCORE_SOFTMAX && (wide || !a.renormalise)) {
-            m = l[0];
+    } else {
 #pragma unroll
-            for (int i = 1; i < VPL; ++i) m = fmaxf(m, l[i]);
-            m = lanes_max<LPT>(m);
-            if (m == -INFINITY) m = 0.0f;
-            md = m;
-        }
-        if constexpr (wide) {
-            double p[VPL];
-            if (a.score == EIF_HIP_SCORE_SOFTMAX) {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) {
-                    p[i] = exp((double)l[i] - md);   // e^-inf = 0 where shut out
-                    zd += p[i];
-                }
-                zd = lanes_sum<LPT>(zd);
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) p[i] /= zd;
-            } else {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) p[i] = 1.0 / (1.0 + exp(-(double)l[i]));
-            }
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const int e = i * LPT + sub;
-                const double b = a.bias && e < a.experts ? (double)a.bias[e] : 0.0;
-                const bool open = l[i] > -INFINITY && b > -INFINITY;
-                p[i] = open ? p[i] + b : none;
-                by[i] = !open ? none : a.bias ? p[i] : (double)l[i];
-                if (a.groups > 1 && e < a.experts) lds[mine * (a.experts + a.groups) + e] = p[i];
-            }
-        } else {
-            if (a.score == EIF_HIP_SCORE_SOFTMAX && !a.renormalise) {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) z += expf(l[i] - m);
-                zd = lanes_sum<LPT>(z);
-            }
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                by[i] = l[i];
-                const int e = i * LPT + sub;
-                if (a.groups > 1 && e < a.experts) reinterpret_cast<KEY *>(lds)[mine * (a.experts + a.groups) + e] = l[i];
-            }
+        for (int i = 0; i < VPL; ++i) {
+            by[i] = l[i];
+            const int e = i * LPT + sub;
+            if (a.groups > 1 && e < a.experts) lds[e] = l[i];
         }
     }
 
     if (a.groups > 1) {
-        KEY *val = reinterpret_cast<KEY *>(lds) + mine * (a.experts + a.groups), *worth = val + a.experts;
+        // lanes that share a group: as many as there are for the power of two of groups
+        KEY *worth = lds + a.experts;
+        int share = 1;
+        while (share * 2 * a.groups <= LPT) share *= 2;
         wave_lds_order();
-        for (int g = sub; g < a.groups; g += LPT) {
+        for (int g0 = 0; g0 < a.groups; g0 += LPT) {
+            const int g = g0 + sub / share, j = sub % share;
             KEY b1 = none, b2 = none;
-            int at = g % a.group_size;   // lanes start at different experts of their groups: different LDS banks
-            for (int j = 0; j < a.group_size; ++j) {
-                const KEY v = val[g * a.group_size + at];
-                at = at + 1 == a.group_size ? 0 : at + 1;
-                if (v > b1) {
-                    b2 = b1;
-                    b1 = v;
-                } else if (v > b2) {
-                    b2 = v;
+            if (g < a.groups) {
+                const KEY *val = lds + g * a.group_size;
+                int at = (j + g * share) % a.group_size;   // lanes start at different experts of their groups: different LDS banks
+                for (int k = j; k < a.group_size; k += share) {
+                    const KEY v = val[at];
+                    at += share;
+                    if (at >= a.group_size) at -= a.group_size;
+                    const bool first = v > b1;
+                    b2 = first ? b1 : larger(b2, v);
+                    b1 = first ? v : b1;
                 }
             }
-            worth[g] = a.best == 2 && b2 > none ? b1 + b2 : b1;
+            butterfly<LPT>([&](auto x) {
+                if (decltype(x)::value < share) {
+                    const KEY o1 = xlane_of<decltype(x)::value>(b1), o2 = xlane_of<decltype(x)::value>(b2);
+                    b2 = larger(o1 > b1 ? b1 : o1, larger(b2, o2));
+                    b1 = larger(b1, o1);
+                }
+            });
+            if (g < a.groups && j == 0) worth[g] = a.best == 2 && b2 > none ? b1 + b2 : b1;
         }
         wave_lds_order();
         uint64_t keep = 0;
@@ -193,52 +286,134 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
             const uint32_t e = i * LPT + sub, g = a.group_size == 1 ? e : __umulhi(e, a.group_magic);
             if (!((keep >> (g & 63)) & 1)) by[i] = none;
         }
+        wave_lds_order();
     }
 
-    int chosen = -1;   // lane k: the token's k-th expert
-    KEY value = none;
-    for (int k = 0; k < a.top; ++k) {
-        KEY best = none;
-        int e = INT32_MAX;
+    KEY *at_value = lds;
+    int *at_expert = reinterpret_cast<int *>(lds + kRoom);
+    float *at_logit = reinterpret_cast<float *>(at_expert + kRoom);
+    KEY floor = by[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            if (by[i] > best) {
-                best = by[i];
-                e = i * LPT + sub;
-            }
+    for (int i = 1; i < VPL; ++i) floor = larger(floor, by[i]);
+    {
+        const KEY v = floor;
+        int above = 0;   // lanes with a larger one
+        if constexpr (LPT == 16) {
+            for_each<1, 15>([&](auto n) { above += row_turn<decltype(n)::value>(v) > v; });
+        } else {
+            KEY *top = lds + route_lds<KEY, LPT>(a.experts, a.groups) - 64;
+            top[sub] = v;
+            wave_lds_order();
+#pragma unroll 16
+            for (int j = 0; j < 64; ++j) above += top[j] > v;
         }
+        floor = above < a.top ? v : (KEY)INFINITY;
         butterfly<LPT>([&](auto x) {
-            const KEY ob = xlane_of<decltype(x)::value>(best);
-            const int oe = __float_as_int(xlane<decltype(x)::value>(__int_as_float(e)));
-            if (ob > best || (ob == best && oe < e)) {
-                best = ob;
-                e = oe;
-            }
+            const KEY o = xlane_of<decltype(x)::value>(floor);
+            floor = o < floor ? o : floor;
         });
-        if (sub == k) {
-            chosen = e == INT32_MAX ? -1 : e;
-            value = best;
-        }
+    }
+    int n = 0;   // candidates, in the order of their experts
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) by[i] = i * LPT + sub == e ? none : by[i];
+    for (int i = 0; i < VPL; ++i) {
+        const bool in = by[i] >= floor && by[i] > none;
+        const uint64_t all = __ballot(in);
+        const uint32_t lo = LPT == 64 ? (uint32_t)all : (uint32_t)(all >> (lane & 48)) & 0xffff, hi = LPT == 64 ? (uint32_t)(all >> 32) : 0;
+        const int before = LPT == 64 ? __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, n)) : n + __popc(lo & ((1u << sub) - 1));
+        if (in && before < kRoom) {
+            at_value[before] = by[i];
+            at_expert[before] = i * LPT + sub;
+            at_logit[before] = l[i];
+        }
+        n += __popc(lo) + __popc(hi);
+    }
+    wave_lds_order();
+    int chosen = -1;   // lane k: the token's k-th expert, and its logit
+    float logit = -INFINITY;
+    if (__ballot(n > kRoom) == 0) {
+        // the candidates that come before each of a lane's, and the chosen ones to their places
+        constexpr int C = kRoom / LPT;
+        int e[C], place[C];
+        float le[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k = sub + c * LPT;
+            place[c] = a.top;
+            if (c > 0 && __ballot(n > c * LPT) == 0) continue;
+            if (k < n) {
+                const KEY v = at_value[k];
+                int before = 0;
+                for (int j = 0; j < n; ++j) {
+                    const KEY o = at_value[j];
+                    before += o > v || (o == v && j < k);
+                }
+                e[c] = at_expert[k], le[c] = at_logit[k], place[c] = before;
+            }
+        }
+        wave_lds_order();
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (place[c] < a.top) at_expert[place[c]] = e[c], at_logit[place[c]] = le[c];
+        wave_lds_order();
+        if (sub < min(a.top, n)) chosen = at_expert[sub], logit = at_logit[sub];
+    } else {
+        for (int k = 0; k < a.top; ++k) {
+            KEY best = none;
+            int e = INT32_MAX;
+            float lb = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                if (by[i] > best) {
+                    best = by[i];
+                    e = i * LPT + sub;
+                    lb = l[i];
+                }
+            }
+            butterfly<LPT>([&](auto x) {
+                constexpr int X = decltype(x)::value;
+                const KEY ob = xlane_of<X>(best);
+                const int oe = (int)xlane_u<X>((uint32_t)e);
+                const float ol = xlane_of<X>(lb);
+                if (ob > best || (ob == best && oe < e)) {
+                    best = ob;
+                    e = oe;
+                    lb = ol;
+                }
+            });
+            if (sub == k && e != INT32_MAX) {
+                chosen = e;
+                logit = lb;
+            }
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) by[i] = i * LPT + sub == e ? none : by[i];
+        }
     }
 
     // the weights, a lane each, in 64 bits
     const bool there = chosen >= 0;
     double w = 0.0;
-    const double l = there ? (wide ? (double)logit_at(a, row + chosen) : (double)value) : -INFINITY;
     if (a.score == EIF_HIP_SCORE_SOFTMAX) {
-        if (a.renormalise) md = lanes_max<LPT>(l);
-        w = there ? exp(l - md) : 0.0;
+        if (a.renormalise) md = lanes_max<LPT>(there ? logit : -INFINITY);
+        w = there ? exp64((double)logit - md) : 0.0;
         if (a.renormalise) zd = lanes_sum<LPT>(w);
     } else {
-        w = there ? 1.0 / (1.0 + exp(-l)) : 0.0;
+        w = there ? sigmoid64(logit) : 0.0;
         zd = a.renormalise ? lanes_sum<LPT>(w) : 1.0;
     }
     if (live && sub < a.top) {
         a.ids[token * a.top + sub] = chosen;
         a.weights[token * a.top + sub] = w > 0.0 ? (float)(w / zd * (double)a.scale) : 0.0f;
     }
+}
+
+template <typename KEY, int LPT, int VPL>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
+{
+    extern __shared__ double route_words[];
+    const int mine = threadIdx.x / LPT;   // of the workgroup's tokens
+    const int64_t token = (int64_t)blockIdx.x * (blockDim.x / LPT) + mine;
+    route_token<KEY, LPT, VPL>(a, token < a.tokens ? token : a.tokens - 1, token < a.tokens, threadIdx.x & 63,
+                               reinterpret_cast<KEY *>(route_words) + mine * route_lds<KEY, LPT>(a.experts, a.groups));
 }
 
 // ---- pairs by expert ----
@@ -418,8 +593,9 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 template <typename KEY, int LPT, int VPL>
 int launch_route_as(const RouteArgs &a, hipStream_t st)
 {
-    const size_t each = a.groups > 1 ? (size_t)(a.experts + a.groups) * sizeof(KEY) : 0;
-    const int threads = each * (256 / LPT) > 65536 ? 64 : 256, per = threads / LPT;
+    const size_t each = route_lds<KEY, LPT>(a.experts, a.groups) * sizeof(KEY);
+    // one wave a workgroup where there are few, so that they spread over the CUs, and where LDS would not hold four
+    const int threads = a.tokens <= 4096 || each * (256 / LPT) > 65536 ? 64 : 256, per = threads / LPT;
     route_kernel<KEY, LPT, VPL><<<(unsigned)eif_ceil_div(a.tokens, per), threads, each * per, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
@@ -428,14 +604,12 @@ int launch_route_as(const RouteArgs &a, hipStream_t st)
 template <typename KEY>
 int launch_route(const RouteArgs &a, hipStream_t st)
 {
-    if (a.experts <= 256 && a.top <= 16 && a.tokens >= 1024) {
+    if (a.experts <= 256 && a.top <= 16) {
         if (a.experts <= 32) return launch_route_as<KEY, 16, 2>(a, st);
         if (a.experts <= 64) return launch_route_as<KEY, 16, 4>(a, st);
         if (a.experts <= 128) return launch_route_as<KEY, 16, 8>(a, st);
         return launch_route_as<KEY, 16, 16>(a, st);
     }
-    if (a.experts <= 64) return launch_route_as<KEY, 64, 1>(a, st);
-    if (a.experts <= 128) return launch_route_as<KEY, 64, 2>(a, st);
     if (a.experts <= 256) return launch_route_as<KEY, 64, 4>(a, st);
     if (a.experts <= 512) return launch_route_as<KEY, 64, 8>(a, st);
     if (a.experts <= 1024) return launch_route_as<KEY, 64, 16>(a, st);
