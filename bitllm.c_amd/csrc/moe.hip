@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/eif_hip_moe.h"
 
@@ -155,239 +156,365 @@ EIF_DEV void load_logits(const T *row, int sub, int experts, float *l)
     for (int i = 0; i < VPL; ++i) l[i] = i * LPT + sub < experts ? logit_of(v[i]) : -INFINITY;
 }
 
+// What experts are compared by: their logits (no bias); score plus bias in 64 bits (experts of equal scores in 32 bits can differ in 64,
+// and which of them is chosen changes the token's result by a whole expert); the same, sifted by sigmoids of 32 bits first.
+enum { kByLogit, kByValue, kSifted };
+
 // Candidates of a token that LDS holds: three a lane, or one.
 constexpr int route_room(int lpt) { return lpt == 16 ? 48 : 64; }
 
-// LDS of a token, in KEYs: what the experts and groups are worth, later the candidates; and the lanes' largest.
-template <typename KEY, int LPT>
+// Bytes of LDS of a token: what the experts and groups are worth, later the candidates; and the lanes' largest. kSifted has the room of
+// kByValue, which takes over where it cannot tell.
+template <int MODE, int LPT>
 __host__ __device__ constexpr int route_lds(int experts, int groups)
 {
-    const int kRoom = LPT == 16 ? 48 : 64;
-    const int both = 2 * kRoom * (int)sizeof(float) / (int)sizeof(KEY) + kRoom;   // a KEY, an index and a logit each
-    const int worth = groups > 1 ? experts + groups : 0;
-    return (both > worth ? both : worth) + (LPT == 64 ? 64 : 0);
+    const int room = route_room(LPT) * 16, worth = (experts + groups) * (MODE == kByLogit ? 4 : 8);
+    return ((room > worth ? room : worth) + (LPT == 64 ? 64 * 8 : 0) + 15) / 16 * 16;
 }
 
-// LPT lanes a token, lane `sub` of them has experts sub, sub + LPT, .. (VPL of them). KEY is what experts are compared by: their
-// logits (float), or score plus bias (double; experts of equal scores in 32 bits can differ in 64, and which of them is chosen
-// changes the token's result by a whole expert).
-//   The choice: the top-th largest of the lanes' largest is at most the top-th largest of all, so that the experts at or above it hold the
-// chosen ones, and are few more. They go to LDS, and each counts those that come before it. Where LDS has no room for them (many
-// equals), the largest is taken top times over.
-template <typename KEY, int LPT, int VPL>
-EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, KEY *lds)
+// Error of a sifting value: the sigmoid's is at most 1.9 2^-23 (exponent and sum rounded to 32 bits, the instructions' exponential and
+// reciprocal an ulp off each), the sum's rounding 2^-24 of it.
+EIF_DEV float sift_error(float v) { return fmaf(fabsf(v), 0x1.02p-24f, 0x1p-22f); }
+
+// The groups whose experts may be chosen, a bit each, from what the experts are worth (val [experts], behind them room for the groups).
+// SIFTED: `sure` says whether the kept ones are worth more than the others beyond any error.
+template <int LPT, bool SIFTED, typename KEY>
+EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
 {
-    constexpr bool wide = sizeof(KEY) == 8;
-    constexpr int kRoom = route_room(LPT);
+    const KEY none = -INFINITY;
+    const int sub = lane % LPT;
+    KEY *worth = val + a.experts;
+    int share = 1;   // lanes that share a group: as many as there are for the power of two of groups
+    while (share * 2 * a.groups <= LPT) share *= 2;
+    wave_lds_order();
+    for (int g0 = 0; g0 < a.groups; g0 += LPT) {
+        const int g = g0 + sub / share, j = sub % share;
+        KEY b1 = none, b2 = none;
+        if (g < a.groups) {
+            const KEY *of = val + g * a.group_size;
+            int at = (j + g * share) % a.group_size;   // lanes start at different experts of their groups: different LDS banks
+#pragma unroll 4
+            for (int k = j; k < a.group_size; k += share) {
+                const KEY v = of[at];
+                at += share;
+                if (at >= a.group_size) at -= a.group_size;
+                const bool first = v > b1;
+                b2 = first ? b1 : larger(b2, v);
+                b1 = first ? v : b1;
+            }
+        }
+        butterfly<LPT>([&](auto x) {
+            if (decltype(x)::value < share) {
+                const KEY o1 = xlane_of<decltype(x)::value>(b1), o2 = xlane_of<decltype(x)::value>(b2);
+                b2 = larger(o1 > b1 ? b1 : o1, larger(b2, o2));
+                b1 = larger(b1, o1);
+            }
+        });
+        if (g < a.groups && j == 0) {
+            const bool both = a.best == 2 && b2 > none;
+            worth[g] = both ? b1 + b2 : b1;
+            if constexpr (SIFTED) worth[a.groups + g] = sift_error(b1) + (both ? sift_error(b2) + fabsf(b1 + b2) * 0x1.02p-24f : 0.0f);
+        }
+    }
+    wave_lds_order();
+    uint64_t keep = 0;
+    KEY kept_least = INFINITY, dropped_most = none;
+    for (int g0 = 0; g0 < a.groups; g0 += LPT) {
+        const int g = g0 + sub;
+        int better = a.kept;
+        if (g < a.groups) {
+            const KEY w = worth[g];
+            better = 0;
+#pragma unroll 4
+            for (int h = 0; h < a.groups; ++h) better += worth[h] > w || (worth[h] == w && h < g);
+            if constexpr (SIFTED) {
+                const float off = worth[a.groups + g];
+                if (better < a.kept) kept_least = fminf(kept_least, w - off);
+                else dropped_most = larger(dropped_most, w + off);
+            }
+        }
+        const uint64_t bits = __ballot(better < a.kept);
+        keep |= LPT == 64 ? bits : ((bits >> (lane & 48)) & 0xffff) << g0;
+    }
+    if constexpr (SIFTED) {
+        const float least = -lanes_max<LPT>(-kept_least), most = lanes_max<LPT>(dropped_most);
+        sure = least > most || !(most > none);
+    }
+    wave_lds_order();
+    return keep;
+}
+
+EIF_DEV int group_of(const RouteArgs &a, uint32_t e) { return a.group_size == 1 ? e : __umulhi(e, a.group_magic); }
+
+EIF_DEV float logit_at(const RouteArgs &a, int64_t i)
+{
+    if (a.type == EIF_HIP_F32) return logit_of(static_cast<const float *>(a.logits)[i]);
+    return a.type == EIF_HIP_F16 ? logit_of(static_cast<const __half *>(a.logits)[i]) : logit_of(static_cast<const __hip_bfloat16 *>(a.logits)[i]);
+}
+
+// What an expert is worth in 64 bits: its score, plus the bias; -inf where it is shut out. md, inverse: softmax.
+EIF_DEV double value_of(const RouteArgs &a, float l, int e, double md, double inverse)
+{
+    const double s = a.score == EIF_HIP_SCORE_SOFTMAX ? (l > -INFINITY ? exp64((double)l - md) * inverse : 0.0) : sigmoid64(l);
+    const double b = a.bias ? (double)a.bias[e] : 0.0;
+    return l > -INFINITY && b > -INFINITY ? s + b : -INFINITY;
+}
+
+// The choice of any number of experts and of any equals: they stay in LDS, and the largest is taken top times over. Lane k gets the k-th.
+template <int LPT, typename KEY>
+EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val, double md, double inverse, int &chosen, float &logit)
+{
+    constexpr bool by_value = sizeof(KEY) == 8;
+    const KEY none = -INFINITY;
+    const int sub = lane % LPT;
+    wave_lds_order();
+#pragma unroll 4
+    for (int e = sub; e < a.experts; e += LPT) {
+        const float l = logit_at(a, row + e);
+        if constexpr (by_value) val[e] = value_of(a, l, e, md, inverse);
+        else val[e] = l;
+    }
+    if (a.groups > 1 || (by_value && !a.bias)) {
+        bool sure;
+        const uint64_t keep = a.groups > 1 ? kept_groups<LPT, false>(a, lane, val, sure) : ~0ull;
+#pragma unroll 1
+        for (int e = sub; e < a.experts; e += LPT) {
+            if (!((keep >> (a.groups > 1 ? group_of(a, e) : 0)) & 1)) val[e] = none;
+            else if (by_value && !a.bias) val[e] = logit_at(a, row + e);   // the groups alone go by the scores
+        }
+    }
+    chosen = -1;
+#pragma unroll 1
+    for (int k = 0; k < a.top; ++k) {
+        wave_lds_order();
+        KEY best = none;
+        int at = INT32_MAX;
+#pragma unroll 4
+        for (int e = sub; e < a.experts; e += LPT) {
+            const KEY v = val[e];
+            at = v > best ? e : at;
+            best = larger(best, v);
+        }
+        butterfly<LPT>([&](auto x) {
+            constexpr int X = decltype(x)::value;
+            const KEY ob = xlane_of<X>(best);
+            const int oe = (int)xlane_u<X>((uint32_t)at);
+            if (ob > best || (ob == best && oe < at)) {
+                best = ob;
+                at = oe;
+            }
+        });
+        if (at == INT32_MAX) continue;
+        if (sub == k) chosen = at;
+        if (at % LPT == sub) val[at] = none;
+    }
+    if (chosen >= 0) logit = logit_at(a, row + chosen);
+}
+
+// LPT lanes a token, lane `sub` of them has experts sub, sub + LPT, .. (VPL of them; 0: any number, chosen plainly).
+//   The choice: the top-th largest of the lanes' largest is at most the top-th largest of all, so that the experts at or above it hold the
+// chosen ones, and are few more. They go to LDS, and each counts those that come before it. Sifted: the candidates are those within
+// the error of 32 bits, and only they are computed in 64, an expert a lane in place of all, or the groups where two of them are nearer to
+// each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly. The instructions bound it.
+template <int MODE, int LPT, int VPL>
+EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, char *lds)
+{
+    typedef typename std::conditional<MODE == kByValue, double, float>::type KEY;
+    typedef typename std::conditional<MODE == kByLogit, float, double>::type VALUE;   // of a candidate
+    constexpr int kRoom = route_room(LPT), kEach = VPL > 0 ? VPL : 1;
     const KEY none = -INFINITY;
     const int sub = lane % LPT;
     const int64_t row = token * a.ldl;
 
-    float l[VPL];
-    KEY by[VPL];
-    if (a.type == EIF_HIP_F32) load_logits<LPT, VPL>(static_cast<const float *>(a.logits) + row, sub, a.experts, l);
-    else if (a.type == EIF_HIP_F16) load_logits<LPT, VPL>(static_cast<const __half *>(a.logits) + row, sub, a.experts, l);
-    else load_logits<LPT, VPL>(static_cast<const __hip_bfloat16 *>(a.logits) + row, sub, a.experts, l);
-    double md = 0.0, zd = 1.0;   // softmax: largest logit, sum of e^(l - m)
-    if (a.score == EIF_HIP_SCORE_SOFTMAX && (wide || !a.renormalise)) {
-        float m = l[0];
-#pragma unroll
-        for (int i = 1; i < VPL; ++i) m = larger(m, l[i]);
-        m = lanes_max<LPT>(m);
-        if (m == -INFINITY) m = 0.0f;
-        md = m;
-        if constexpr (!wide) {
-            float z = 0.0f;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) z += expf(l[i] - m);
-            zd = lanes_sum<LPT>(z);
-        }
-    }
-    if constexpr (wide) {
-        double p[VPL];
-        if (a.score == EIF_HIP_SCORE_SOFTMAX) {
-            zd = 0.0;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                p[i] = l[i] > -INFINITY ? exp64((double)l[i] - md) : 0.0;
-                zd += p[i];
-            }
-            zd = lanes_sum<LPT>(zd);
-            const double inverse = 1.0 / zd;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) p[i] *= inverse;
-        } else {
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) p[i] = sigmoid64(l[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int e = i * LPT + sub;
-            const double b = a.bias && e < a.experts ? (double)a.bias[e] : 0.0;
-            const bool open = l[i] > -INFINITY && b > -INFINITY;
-            p[i] = open ? p[i] + b : none;
-            by[i] = !open ? none : a.bias ? p[i] : (double)l[i];
-            if (a.groups > 1 && e < a.experts) lds[e] = p[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            by[i] = l[i];
-            const int e = i * LPT + sub;
-            if (a.groups > 1 && e < a.experts) lds[e] = l[i];
-        }
-    }
-
-    if (a.groups > 1) {
-        // lanes that share a group: as many as there are for the power of two of groups
-        KEY *worth = lds + a.experts;
-        int share = 1;
-        while (share * 2 * a.groups <= LPT) share *= 2;
-        wave_lds_order();
-        for (int g0 = 0; g0 < a.groups; g0 += LPT) {
-            const int g = g0 + sub / share, j = sub % share;
-            KEY b1 = none, b2 = none;
-            if (g < a.groups) {
-                const KEY *val = lds + g * a.group_size;
-                int at = (j + g * share) % a.group_size;   // lanes start at different experts of their groups: different LDS banks
-                for (int k = j; k < a.group_size; k += share) {
-                    const KEY v = val[at];
-                    at += share;
-                    if (at >= a.group_size) at -= a.group_size;
-                    const bool first = v > b1;
-                    b2 = first ? b1 : larger(b2, v);
-                    b1 = first ? v : b1;
-                }
-            }
-            butterfly<LPT>([&](auto x) {
-                if (decltype(x)::value < share) {
-                    const KEY o1 = xlane_of<decltype(x)::value>(b1), o2 = xlane_of<decltype(x)::value>(b2);
-                    b2 = larger(o1 > b1 ? b1 : o1, larger(b2, o2));
-                    b1 = larger(b1, o1);
-                }
-            });
-            if (g < a.groups && j == 0) worth[g] = a.best == 2 && b2 > none ? b1 + b2 : b1;
-        }
-        wave_lds_order();
-        uint64_t keep = 0;
-        for (int g0 = 0; g0 < a.groups; g0 += LPT) {
-            const int g = g0 + sub;
-            int better = a.kept;
-            if (g < a.groups) {
-                const KEY w = worth[g];
-                better = 0;
-                for (int h = 0; h < a.groups; ++h) better += worth[h] > w || (worth[h] == w && h < g);
-            }
-            const uint64_t bits = __ballot(better < a.kept);
-            keep |= LPT == 64 ? bits : ((bits >> (lane & 48)) & 0xffff) << g0;
-        }
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const uint32_t e = i * LPT + sub, g = a.group_size == 1 ? e : __umulhi(e, a.group_magic);
-            if (!((keep >> (g & 63)) & 1)) by[i] = none;
-        }
-        wave_lds_order();
-    }
-
-    KEY *at_value = lds;
-    int *at_expert = reinterpret_cast<int *>(lds + kRoom);
-    float *at_logit = reinterpret_cast<float *>(at_expert + kRoom);
-    KEY floor = by[0];
-#pragma unroll
-    for (int i = 1; i < VPL; ++i) floor = larger(floor, by[i]);
-    {
-        const KEY v = floor;
-        int above = 0;   // lanes with a larger one
-        if constexpr (LPT == 16) {
-            for_each<1, 15>([&](auto n) { above += row_turn<decltype(n)::value>(v) > v; });
-        } else {
-            KEY *top = lds + route_lds<KEY, LPT>(a.experts, a.groups) - 64;
-            top[sub] = v;
-            wave_lds_order();
-#pragma unroll 16
-            for (int j = 0; j < 64; ++j) above += top[j] > v;
-        }
-        floor = above < a.top ? v : (KEY)INFINITY;
-        butterfly<LPT>([&](auto x) {
-            const KEY o = xlane_of<decltype(x)::value>(floor);
-            floor = o < floor ? o : floor;
-        });
-    }
-    int n = 0;   // candidates, in the order of their experts
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const bool in = by[i] >= floor && by[i] > none;
-        const uint64_t all = __ballot(in);
-        const uint32_t lo = LPT == 64 ? (uint32_t)all : (uint32_t)(all >> (lane & 48)) & 0xffff, hi = LPT == 64 ? (uint32_t)(all >> 32) : 0;
-        const int before = LPT == 64 ? __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, n)) : n + __popc(lo & ((1u << sub) - 1));
-        if (in && before < kRoom) {
-            at_value[before] = by[i];
-            at_expert[before] = i * LPT + sub;
-            at_logit[before] = l[i];
-        }
-        n += __popc(lo) + __popc(hi);
-    }
-    wave_lds_order();
     int chosen = -1;   // lane k: the token's k-th expert, and its logit
     float logit = -INFINITY;
-    if (__ballot(n > kRoom) == 0) {
-        // the candidates that come before each of a lane's, and the chosen ones to their places
-        constexpr int C = kRoom / LPT;
-        int e[C], place[C];
-        float le[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int k = sub + c * LPT;
-            place[c] = a.top;
-            if (c > 0 && __ballot(n > c * LPT) == 0) continue;
-            if (k < n) {
-                const KEY v = at_value[k];
-                int before = 0;
-                for (int j = 0; j < n; ++j) {
-                    const KEY o = at_value[j];
-                    before += o > v || (o == v && j < k);
-                }
-                e[c] = at_expert[k], le[c] = at_logit[k], place[c] = before;
+    bool plainly = VPL == 0;
+    double md = 0.0, zd = 1.0;   // softmax: largest logit, sum of e^(l - m)
+    const bool over_all = a.score == EIF_HIP_SCORE_SOFTMAX && (MODE == kByValue || !a.renormalise);
+    if constexpr (VPL == 0) {
+        if (over_all) {
+            float m = -INFINITY;
+#pragma unroll 4
+            for (int e = sub; e < a.experts; e += LPT) m = larger(m, logit_at(a, row + e));
+            m = lanes_max<LPT>(m);
+            md = m == -INFINITY ? 0.0f : m;
+            zd = 0.0;
+#pragma unroll 2
+            for (int e = sub; e < a.experts; e += LPT) {
+                const float l = logit_at(a, row + e);
+                zd += l > -INFINITY ? exp64((double)l - md) : 0.0;
             }
+            zd = lanes_sum<LPT>(zd);
         }
-        wave_lds_order();
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (place[c] < a.top) at_expert[place[c]] = e[c], at_logit[place[c]] = le[c];
-        wave_lds_order();
-        if (sub < min(a.top, n)) chosen = at_expert[sub], logit = at_logit[sub];
     } else {
-        for (int k = 0; k < a.top; ++k) {
-            KEY best = none;
-            int e = INT32_MAX;
-            float lb = -INFINITY;
+        float l[kEach];
+        KEY by[kEach];
+        if (a.type == EIF_HIP_F32) load_logits<LPT, kEach>(static_cast<const float *>(a.logits) + row, sub, a.experts, l);
+        else if (a.type == EIF_HIP_F16) load_logits<LPT, kEach>(static_cast<const __half *>(a.logits) + row, sub, a.experts, l);
+        else load_logits<LPT, kEach>(static_cast<const __hip_bfloat16 *>(a.logits) + row, sub, a.experts, l);
+        if (over_all) {
+            float m = l[0];
+#pragma unroll
+            for (int i = 1; i < VPL; ++i) m = larger(m, l[i]);
+            m = lanes_max<LPT>(m);
+            md = m == -INFINITY ? 0.0f : m;
+        }
+        KEY *val = reinterpret_cast<KEY *>(lds);
+        if constexpr (MODE == kByValue) {
+            double p[kEach];
+            if (a.score == EIF_HIP_SCORE_SOFTMAX) {
+                zd = 0.0;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) {
+                    p[i] = l[i] > -INFINITY ? exp64((double)l[i] - md) : 0.0;
+                    zd += p[i];
+                }
+                zd = lanes_sum<LPT>(zd);
+                const double inverse = 1.0 / zd;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) p[i] *= inverse;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) p[i] = sigmoid64(l[i]);
+            }
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
-                if (by[i] > best) {
-                    best = by[i];
-                    e = i * LPT + sub;
-                    lb = l[i];
-                }
+                const int e = i * LPT + sub;
+                const double b = a.bias && e < a.experts ? (double)a.bias[e] : 0.0;
+                const bool open = l[i] > -INFINITY && b > -INFINITY;
+                p[i] = open ? p[i] + b : none;
+                by[i] = !open ? none : a.bias ? p[i] : (double)l[i];
+                if (a.groups > 1 && e < a.experts) val[e] = p[i];
             }
-            butterfly<LPT>([&](auto x) {
-                constexpr int X = decltype(x)::value;
-                const KEY ob = xlane_of<X>(best);
-                const int oe = (int)xlane_u<X>((uint32_t)e);
-                const float ol = xlane_of<X>(lb);
-                if (ob > best || (ob == best && oe < e)) {
-                    best = ob;
-                    e = oe;
-                    lb = ol;
-                }
-            });
-            if (sub == k && e != INT32_MAX) {
-                chosen = e;
-                logit = lb;
+        } else if constexpr (MODE == kSifted) {
+            float b[kEach];
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) b[i] = a.bias[min(i * LPT + sub, a.experts - 1)];
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const int e = i * LPT + sub;
+                const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[i] * -1.44269504f));
+                const float v = fmaf(l[i], 0.0f, s + b[i]);   // a logit of -inf makes it NaN
+                by[i] = v > none ? v : none;
+                if (a.groups > 1 && e < a.experts) val[e] = by[i];
+            }
+        } else {
+            if (over_all) {
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) z += expf(l[i] - (float)md);
+                zd = lanes_sum<LPT>(z);
             }
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) by[i] = i * LPT + sub == e ? none : by[i];
+            for (int i = 0; i < VPL; ++i) {
+                by[i] = l[i];
+                const int e = i * LPT + sub;
+                if (a.groups > 1 && e < a.experts) val[e] = l[i];
+            }
+        }
+
+        if (a.groups > 1) {
+            bool sure = true;
+            uint64_t keep = kept_groups<LPT, MODE == kSifted>(a, lane, val, sure);
+            if constexpr (MODE == kSifted) {
+                if (__ballot(!sure)) {   // 64 bits tell
+                    double *value = reinterpret_cast<double *>(lds);
+#pragma unroll 4
+                    for (int e = sub; e < a.experts; e += LPT) value[e] = value_of(a, logit_at(a, row + e), e, 0.0, 1.0);
+                    keep = kept_groups<LPT, false>(a, lane, value, sure);
+                }
+            }
+            if (a.group_size % LPT == 0) {   // a lane's i-th expert is of the same group in every lane
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (!((keep >> (i * LPT / a.group_size & 63)) & 1)) by[i] = none;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (!((keep >> (group_of(a, i * LPT + sub) & 63)) & 1)) by[i] = none;
+            }
+        }
+
+        VALUE *at_value = reinterpret_cast<VALUE *>(lds);
+        int *at_expert = reinterpret_cast<int *>(lds + kRoom * 8);
+        float *at_logit = reinterpret_cast<float *>(at_expert + kRoom);
+        KEY floor = by[0];
+#pragma unroll
+        for (int i = 1; i < VPL; ++i) floor = larger(floor, by[i]);
+        {
+            const KEY v = floor;
+            int above = 0;   // lanes with a larger one
+            if constexpr (LPT == 16) {
+                for_each<1, 15>([&](auto n) { above += row_turn<decltype(n)::value>(v) > v; });
+            } else {
+                KEY *top = reinterpret_cast<KEY *>(lds + route_lds<MODE, LPT>(a.experts, a.groups) - 64 * 8);
+                top[sub] = v;
+                wave_lds_order();
+#pragma unroll 16
+                for (int j = 0; j < 64; ++j) above += top[j] > v;
+            }
+            floor = above < a.top ? v : (KEY)INFINITY;
+            butterfly<LPT>([&](auto x) {
+                const KEY o = xlane_of<decltype(x)::value>(floor);
+                floor = o < floor ? o : floor;
+            });
+            if constexpr (MODE == kSifted) floor = floor < INFINITY ? floor - 2.0f * sift_error(floor) : floor;
+        }
+        int n = 0;   // candidates, in the order of their experts
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const bool in = by[i] >= floor && by[i] > none;
+            const uint64_t all = __ballot(in);
+            const uint32_t lo = LPT == 64 ? (uint32_t)all : (uint32_t)(all >> (lane & 48)) & 0xffff, hi = LPT == 64 ? (uint32_t)(all >> 32) : 0;
+            const int before = LPT == 64 ? __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, n)) : n + __popc(lo & ((1u << sub) - 1));
+            if (in && before < kRoom) {
+                if constexpr (MODE != kSifted) at_value[before] = by[i];
+                at_expert[before] = i * LPT + sub;
+                at_logit[before] = l[i];
+            }
+            n += __popc(lo) + __popc(hi);
+        }
+        wave_lds_order();
+        plainly = plainly || __ballot(n > kRoom) != 0;
+        if (!plainly) {
+            // the candidates that come before each of a lane's, and the chosen ones to their places
+            constexpr int C = kRoom / LPT;
+            int e[C], place[C];
+            float le[C];
+            VALUE v[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int k = sub + c * LPT;
+                place[c] = a.top;
+                if (k < n) {
+                    e[c] = at_expert[k], le[c] = at_logit[k];
+                    if constexpr (MODE == kSifted) at_value[k] = v[c] = sigmoid64(le[c]) + (double)a.bias[e[c]];
+                    else v[c] = at_value[k];
+                }
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int k = sub + c * LPT;
+                if (k < n) {
+                    int before = 0;
+#pragma unroll 4
+                    for (int j = 0; j < n; ++j) {
+                        const VALUE o = at_value[j];
+                        before += o > v[c] || (o == v[c] && j < k);
+                    }
+                    place[c] = before;
+                }
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (place[c] < a.top) at_expert[place[c]] = e[c], at_logit[place[c]] = le[c];
+            wave_lds_order();
+            if (sub < min(a.top, n)) chosen = at_expert[sub], logit = at_logit[sub];
         }
     }
+    if (plainly) choose_plainly<LPT>(a, row, lane, reinterpret_cast<VALUE *>(lds), md, 1.0 / zd, chosen, logit);
 
     // the weights, a lane each, in 64 bits
     const bool there = chosen >= 0;
@@ -406,28 +533,38 @@ EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane,
     }
 }
 
-template <typename KEY, int LPT, int VPL>
+template <int MODE, int LPT, int VPL>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
 {
-    extern __shared__ double route_words[];
+    extern __shared__ char route_bytes[];
     const int mine = threadIdx.x / LPT;   // of the workgroup's tokens
     const int64_t token = (int64_t)blockIdx.x * (blockDim.x / LPT) + mine;
-    route_token<KEY, LPT, VPL>(a, token < a.tokens ? token : a.tokens - 1, token < a.tokens, threadIdx.x & 63,
-                               reinterpret_cast<KEY *>(route_words) + mine * route_lds<KEY, LPT>(a.experts, a.groups));
+    route_token<MODE, LPT, VPL>(a, token < a.tokens ? token : a.tokens - 1, token < a.tokens, threadIdx.x & 63,
+                                route_bytes + mine * route_lds<MODE, LPT>(a.experts, a.groups));
 }
 
 // ---- pairs by expert ----
 
 constexpr int kSortBlocks = 256;      // of a sort in two launches, at most: one a CU
-constexpr int kSortAlone = 8192;      // pairs that one workgroup sorts in one launch
-constexpr int kSortStep = 4096;       // pairs of a workgroup at least, in two launches
+// Pairs that one workgroup sorts in one launch: a thousand more take it a microsecond (4000 of 64 experts 6.3 us, 8000 of 128 10.6), two
+// launches take 6.6 and 8.3 us there.
+constexpr int kSortAlone = 4096;
+constexpr int kHeld = 4;              // of a wave's runs of 64 pairs, in registers
 
-// Waves of a placing workgroup: each has a counter of every expert in LDS, 64 KB in all.
-int sort_waves(int experts) { return experts > 2048 ? 2 : experts > 1024 ? 4 : experts > 512 ? 8 : 16; }
-// Pairs of a workgroup, whole steps of its waves, and how many workgroups that takes.
+// Waves of a placing workgroup: one for 64 pairs, up to 16 with a counter of every expert in LDS each, 64 KB in all.
+int sort_waves(int experts, int pairs)
+{
+    int waves = experts > 2048 ? 2 : experts > 1024 ? 4 : experts > 512 ? 8 : 16;
+    while (waves > 1 && (waves / 2) * 64 >= pairs) waves /= 2;
+    return waves;
+}
+// Pairs of a workgroup, whole steps of its waves: 1024, more from 128 workgroups on, whose counts each of them adds up (us of both
+// launches with 1024 / 2048 / 4096: 16384 pairs of 64 experts 8.0 / 9.0 / -; 65536 of 256 9.5 / 9.8 / 12.4; 262144 of 128 11.4 / 10.7 /
+// 11.7).
 int sort_share(int64_t pairs)
 {
-    const int64_t per = std::max<int64_t>(kSortStep, (pairs + kSortBlocks - 1) / kSortBlocks);
+    int64_t per = std::min<int64_t>((pairs + 127) / 128, 4096);
+    per = std::max<int64_t>({per, 1024, (pairs + kSortBlocks - 1) / kSortBlocks});
     return (int)((per + 1023) / 1024 * 1024);
 }
 int sort_blocks(int64_t pairs) { return pairs <= kSortAlone ? 1 : (int)((pairs + sort_share(pairs) - 1) / sort_share(pairs)); }
@@ -463,34 +600,55 @@ EIF_DEV uint64_t same_id(int id, bool live, int bits)
 __global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, int pairs, int share, int experts, int bits, int top,
                                                           const int32_t *counts, int blocks, int32_t *offsets, int32_t *row, int32_t *slot)
 {
-    extern __shared__ int32_t cnt[];   // [waves][experts], then the sums [experts] and of the waves [16]
+    extern __shared__ int32_t cnt[];   // [waves][experts], then the sums [experts], those of workgroups before [experts], and of the waves [16]
     const int threads = blockDim.x, waves = threads >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int32_t *sums = cnt + waves * experts, *part = sums + experts;
+    int32_t *sums = cnt + waves * experts, *before = sums + experts, *part = before + experts;
     int32_t *own = cnt + wave * experts;
     const int lo = blockIdx.x * share, n = min(pairs - lo, share), run = (n + waves * 64 - 1) / (waves * 64) * 64;
-    for (int i = threadIdx.x; i < waves * experts; i += threads) cnt[i] = 0;
-    __syncthreads();
     const int from = min(wave * run, n), to = min(from + run, n);
-    for (int i = from + lane; i < to; i += 64) {
+    int held[kHeld];   // the wave's first pairs stay in registers
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+        const int i = from + h * 64 + lane;
+        held[h] = i < to ? ids[lo + i] : -1;
+    }
+    for (int i = threadIdx.x; i < (waves + 2) * experts; i += threads) cnt[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+        if ((unsigned)held[h] < (unsigned)experts) atomicAdd(&own[held[h]], 1);
+    for (int i = from + kHeld * 64 + lane; i < to; i += 64) {
         const int id = ids[lo + i];
         if ((unsigned)id < (unsigned)experts) atomicAdd(&own[id], 1);
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += threads) {
-        int before = 0, all = 0;
-        if (blocks > 1) {
-            for (int b = 0; b < blocks; ++b) {
+    if (blocks > 1) {
+        // the other workgroups' counts: all threads at once, eight loads of each under way (one thread an expert, a load after the
+        // other, took 12 of 21 us with 64 workgroups and 128 experts)
+        const int parts = max(1, threads / experts), per = (blocks + parts - 1) / parts;
+        for (int i = threadIdx.x; i < parts * experts; i += threads) {
+            const int p = i / experts, e = i - p * experts, b1 = min((p + 1) * per, blocks);
+            int first = 0, all = 0;
+#pragma unroll 8
+            for (int b = p * per; b < b1; ++b) {
                 const int c = counts[b * experts + e];
-                before += b < (int)blockIdx.x ? c : 0;
+                first += b < (int)blockIdx.x ? c : 0;
                 all += c;
             }
+            atomicAdd(&before[e], first);
+            atomicAdd(&sums[e], all);
         }
-        for (int w = 0; w < waves; ++w) {
-            const int c = cnt[w * experts + e];
-            cnt[w * experts + e] = before;
-            before += c;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += threads) {
+        int at = before[e], c[16];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) c[w] = w < waves ? cnt[w * experts + e] : 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < waves) cnt[w * experts + e] = at;
+            at += c[w];
         }
-        sums[e] = blocks > 1 ? all : before;
+        if (blocks == 1) sums[e] = at;
     }
     __syncthreads();
     // exclusive sums over the experts: each thread's run of them, the wave's, the workgroup's
@@ -515,9 +673,8 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, in
         if (blockIdx.x == 0 && e == experts - 1) offsets[experts] = at;
     }
     __syncthreads();
-    for (int i = from; i < to; i += 64) {
+    const auto place = [&](int i, int id) {
         const int p = lo + i + lane;
-        const int id = i + lane < to ? ids[p] : -1;
         const bool live = (unsigned)id < (unsigned)experts;
         const uint64_t same = same_id(id, live, bits);
         int place = -1;
@@ -529,7 +686,11 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, in
         wave_lds_order();
         if (live && (same >> lane) == 1) own[id] += __popcll(same);   // the last of the lanes that share an id
         wave_lds_order();
-    }
+    };
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+        if (from + h * 64 < to) place(from + h * 64, held[h]);
+    for (int i = from + kHeld * 64; i < to; i += 64) place(i, i + lane < to ? ids[lo + i + lane] : -1);
 }
 
 // ---- the experts' rows together ----
@@ -590,30 +751,34 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 
 // ---- launches ----
 
-template <typename KEY, int LPT, int VPL>
+template <int MODE, int LPT, int VPL>
 int launch_route_as(const RouteArgs &a, hipStream_t st)
 {
-    const size_t each = route_lds<KEY, LPT>(a.experts, a.groups) * sizeof(KEY);
+    const size_t each = route_lds<MODE, LPT>(a.experts, a.groups);
     // one wave a workgroup where there are few, so that they spread over the CUs, and where LDS would not hold four
     const int threads = a.tokens <= 4096 || each * (256 / LPT) > 65536 ? 64 : 256, per = threads / LPT;
-    route_kernel<KEY, LPT, VPL><<<(unsigned)eif_ceil_div(a.tokens, per), threads, each * per, st>>>(a);
+    route_kernel<MODE, LPT, VPL><<<(unsigned)eif_ceil_div(a.tokens, per), threads, each * per, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
 
-template <typename KEY>
+template <int MODE>
 int launch_route(const RouteArgs &a, hipStream_t st)
 {
     if (a.experts <= 256 && a.top <= 16) {
-        if (a.experts <= 32) return launch_route_as<KEY, 16, 2>(a, st);
-        if (a.experts <= 64) return launch_route_as<KEY, 16, 4>(a, st);
-        if (a.experts <= 128) return launch_route_as<KEY, 16, 8>(a, st);
-        return launch_route_as<KEY, 16, 16>(a, st);
+        if (a.experts <= 32) return launch_route_as<MODE, 16, 2>(a, st);
+        if (a.experts <= 64) return launch_route_as<MODE, 16, 4>(a, st);
+        if (a.experts <= 128) return launch_route_as<MODE, 16, 8>(a, st);
+        return launch_route_as<MODE, 16, 16>(a, st);
     }
-    if (a.experts <= 256) return launch_route_as<KEY, 64, 4>(a, st);
-    if (a.experts <= 512) return launch_route_as<KEY, 64, 8>(a, st);
-    if (a.experts <= 1024) return launch_route_as<KEY, 64, 16>(a, st);
-    return launch_route_as<KEY, 64, 64>(a, st);
+    if constexpr (MODE == kSifted) {
+        return launch_route<kByValue>(a, st);
+    } else {
+        if (a.experts <= 256) return launch_route_as<MODE, 64, 4>(a, st);
+        if (a.experts <= 512) return launch_route_as<MODE, 64, 8>(a, st);
+        if (a.experts <= 1024) return launch_route_as<MODE, 64, 16>(a, st);
+        return launch_route_as<MODE, 64, 0>(a, st);
+    }
 }
 
 // Arguments of a sort; EIF_HIP_OK where it may be launched.
@@ -639,8 +804,8 @@ int launch_sort(const int32_t *ids, int tokens, int top, int experts, int32_t *o
         sort_count_kernel<<<blocks, 1024, experts * sizeof(int32_t), st>>>(ids, pairs, share, experts, counts);
         EIF_HIP_LAUNCHED();
     }
-    const int waves = sort_waves(experts);
-    const size_t lds = ((size_t)(waves + 1) * experts + 16) * sizeof(int32_t);
+    const int waves = sort_waves(experts, share);
+    const size_t lds = ((size_t)(waves + 2) * experts + 16) * sizeof(int32_t);
     sort_place_kernel<<<blocks, 64 * waves, lds, st>>>(ids, pairs, share, experts, bits, top, counts, blocks, offsets, row, slot);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
@@ -704,8 +869,8 @@ int eif_hip_moe_route(const void *logits, int type, int64_t ldl, int tokens, con
         a.groups = s.groups_kept < s.groups ? s.groups : 1, a.kept = s.groups_kept, a.best = s.group_best;
         a.group_size = s.experts / s.groups;
         a.group_magic = (uint32_t)((0xffffffffull + a.group_size) / a.group_size);
-        const bool wide = s.bias || (a.groups > 1 && a.best == 2);
-        const int rc = wide ? launch_route<double>(a, st) : launch_route<float>(a, st);
+        const bool by_value = s.bias || (a.groups > 1 && a.best == 2), sifted = s.bias && s.score == EIF_HIP_SCORE_SIGMOID;
+        const int rc = sifted ? launch_route<kSifted>(a, st) : by_value ? launch_route<kByValue>(a, st) : launch_route<kByLogit>(a, st);
         if (rc) return rc;
     }
     return sorted ? launch_sort(ids, tokens, s.top_k, s.experts, offsets, row, slot, work, st) : EIF_HIP_OK;
