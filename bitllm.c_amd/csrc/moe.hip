@@ -150,10 +150,17 @@ template <int LPT, int VPL, typename T>
 EIF_DEV void load_logits(const T *row, int sub, int experts, float *l)
 {
     T v[VPL];
+    if (experts == LPT * VPL) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) v[i] = row[min(i * LPT + sub, experts - 1)];
+        for (int i = 0; i < VPL; ++i) v[i] = row[i * LPT + sub];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) l[i] = i * LPT + sub < experts ? logit_of(v[i]) : -INFINITY;
+        for (int i = 0; i < VPL; ++i) l[i] = logit_of(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) v[i] = row[min(i * LPT + sub, experts - 1)];
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) l[i] = i * LPT + sub < experts ? logit_of(v[i]) : -INFINITY;
+    }
 }
 
 // What experts are compared by: their logits (no bias); score plus bias in 64 bits (experts of equal scores in 32 bits can differ in 64,
@@ -597,10 +604,10 @@ EIF_DEV uint64_t same_id(int id, bool live, int bits)
 
 // A workgroup places the pairs [blockIdx share, + share): a pair's place is the pairs of lower experts, those of its expert in
 // workgroups, waves and steps before, and in the lanes before. Each wave has a run of the pairs in order, and counters of its own.
-__global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, int pairs, int share, int experts, int bits, int top,
-                                                          const int32_t *counts, int blocks, int32_t *offsets, int32_t *row, int32_t *slot)
+// cnt: [waves][experts], then the sums [experts], those of workgroups before [experts], and of the waves [16].
+EIF_DEV void sort_place(const int32_t *ids, int pairs, int share, int experts, int bits, int top, const int32_t *counts, int blocks,
+                        int32_t *offsets, int32_t *row, int32_t *slot, int32_t *cnt)
 {
-    extern __shared__ int32_t cnt[];   // [waves][experts], then the sums [experts], those of workgroups before [experts], and of the waves [16]
     const int threads = blockDim.x, waves = threads >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int32_t *sums = cnt + waves * experts, *before = sums + experts, *part = before + experts;
     int32_t *own = cnt + wave * experts;
@@ -693,6 +700,27 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, in
     for (int i = from + kHeld * 64; i < to; i += 64) place(i, i + lane < to ? ids[lo + i + lane] : -1);
 }
 
+__global__ __launch_bounds__(1024) void sort_place_kernel(const int32_t *ids, int pairs, int share, int experts, int bits, int top,
+                                                          const int32_t *counts, int blocks, int32_t *offsets, int32_t *row, int32_t *slot)
+{
+    extern __shared__ int32_t sort_words[];
+    sort_place(ids, pairs, share, experts, bits, top, counts, blocks, offsets, row, slot, sort_words);
+}
+
+// A few tokens: one workgroup chooses for all of them at once and sorts what it chose, one launch in place of two: one token of 32
+// experts 4.7 us in place of 2.5 and 2.8, 64 of 64 7.3 in place of 4.3 and 4.0.
+template <int MODE, int LPT, int VPL>
+__global__ __launch_bounds__(1024) void route_sort_kernel(RouteArgs a, int bits, int32_t *offsets, int32_t *row, int32_t *slot)
+{
+    extern __shared__ char route_bytes[];
+    const int64_t token = threadIdx.x / LPT;
+    route_token<MODE, LPT, VPL>(a, token < a.tokens ? token : a.tokens - 1, token < a.tokens, threadIdx.x & 63,
+                                route_bytes + token * route_lds<MODE, LPT>(a.experts, a.groups));
+    __syncthreads();   // the ids are in memory for the workgroup's other waves
+    const int pairs = a.tokens * a.top;
+    sort_place(a.ids, pairs, pairs, a.experts, bits, a.top, nullptr, 1, offsets, row, slot, reinterpret_cast<int32_t *>(route_bytes));
+}
+
 // ---- the experts' rows together ----
 
 template <typename T>
@@ -751,34 +779,75 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 
 // ---- launches ----
 
-template <int MODE, int LPT, int VPL>
-int launch_route_as(const RouteArgs &a, hipStream_t st)
+int bits_of(int experts)
 {
-    const size_t each = route_lds<MODE, LPT>(a.experts, a.groups);
-    // one wave a workgroup where there are few, so that they spread over the CUs, and where LDS would not hold four
-    const int threads = a.tokens <= 4096 || each * (256 / LPT) > 65536 ? 64 : 256, per = threads / LPT;
-    route_kernel<MODE, LPT, VPL><<<(unsigned)eif_ceil_div(a.tokens, per), threads, each * per, st>>>(a);
+    int bits = 0;
+    while (1 << bits < experts) ++bits;
+    return bits;
+}
+
+// LDS of a placing workgroup.
+size_t sort_lds(int waves, int experts) { return ((size_t)(waves + 2) * experts + 16) * sizeof(int32_t); }
+
+// Where the sorted pairs of a choice go; offsets NULL: nowhere.
+struct SortedTo {
+    int32_t *offsets, *row, *slot;
+    void *work;
+};
+
+int launch_sort(const int32_t *ids, int tokens, int top, int experts, const SortedTo &to, hipStream_t st)
+{
+    const int pairs = tokens * top, blocks = sort_blocks(pairs), share = blocks > 1 ? sort_share(pairs) : pairs;
+    int32_t *counts = static_cast<int32_t *>(to.work);
+    if (blocks > 1) {
+        sort_count_kernel<<<blocks, 1024, experts * sizeof(int32_t), st>>>(ids, pairs, share, experts, counts);
+        EIF_HIP_LAUNCHED();
+    }
+    const int waves = sort_waves(experts, share);
+    sort_place_kernel<<<blocks, 64 * waves, sort_lds(waves, experts), st>>>(ids, pairs, share, experts, bits_of(experts), top, counts, blocks,
+                                                                            to.offsets, to.row, to.slot);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
 
-template <int MODE>
-int launch_route(const RouteArgs &a, hipStream_t st)
+template <int MODE, int LPT, int VPL>
+int launch_route_as(const RouteArgs &a, const SortedTo &to, hipStream_t st)
 {
-    if (a.experts <= 256 && a.top <= 16) {
-        if (a.experts <= 32) return launch_route_as<MODE, 16, 2>(a, st);
-        if (a.experts <= 64) return launch_route_as<MODE, 16, 4>(a, st);
-        if (a.experts <= 128) return launch_route_as<MODE, 16, 8>(a, st);
-        return launch_route_as<MODE, 16, 16>(a, st);
+    const size_t each = route_lds<MODE, LPT>(a.experts, a.groups);
+    if constexpr (VPL > 0) {
+        // one launch with the sort where one workgroup's waves have room for every token and its counters; not with 16 waves of 64 lanes
+        // a token, whose time on one CU passes that of two launches (16 tokens of 256 experts 11.0 us, 6.1 and 3.5 on many)
+        const int waves = eif_ceil_div(a.tokens, 64 / LPT);
+        const size_t lds = std::max(each * std::min(waves, 16) * (64 / LPT), sort_lds(std::min(waves, 16), a.experts));
+        if (to.offsets && waves <= (LPT == 16 ? 16 : 8) && lds <= 65536) {
+            route_sort_kernel<MODE, LPT, VPL><<<1, 64 * waves, lds, st>>>(a, bits_of(a.experts), to.offsets, to.row, to.slot);
+            EIF_HIP_LAUNCHED();
+            return EIF_HIP_OK;
+        }
     }
-    if constexpr (MODE == kSifted) {
-        return launch_route<kByValue>(a, st);
-    } else {
-        if (a.experts <= 256) return launch_route_as<MODE, 64, 4>(a, st);
-        if (a.experts <= 512) return launch_route_as<MODE, 64, 8>(a, st);
-        if (a.experts <= 1024) return launch_route_as<MODE, 64, 16>(a, st);
-        return launch_route_as<MODE, 64, 0>(a, st);
+    // one wave a workgroup where there are few, so that they spread over the CUs, and where LDS would not hold four
+    const int threads = a.tokens <= 4096 || each * (256 / LPT) > 65536 ? 64 : 256, per = threads / LPT;
+    route_kernel<MODE, LPT, VPL><<<(unsigned)eif_ceil_div(a.tokens, per), threads, each * per, st>>>(a);
+    EIF_HIP_LAUNCHED();
+    return to.offsets ? launch_sort(a.ids, a.tokens, a.top, a.experts, to, st) : EIF_HIP_OK;
+}
+
+// Lanes of a token: 16, so that its fixed work is shared by four tokens of a wave, or 64 where there are few tokens, whose time is one
+// wave's (us, 16 / 64: 64 tokens of 256 experts with a bias and groups 8.9 / 6.5, without 6.9 / 4.8; 2000 9.0 / 7.2, 4000 9.3 / 9.7;
+// one token of 32 3.0 / 3.5).
+template <int MODE>
+int launch_route(const RouteArgs &a, const SortedTo &to, hipStream_t st)
+{
+    if (a.experts <= (a.tokens <= 2048 ? 64 : 256) && a.top <= 16) {
+        if (a.experts <= 32) return launch_route_as<MODE, 16, 2>(a, to, st);
+        if (a.experts <= 64) return launch_route_as<MODE, 16, 4>(a, to, st);
+        if (a.experts <= 128) return launch_route_as<MODE, 16, 8>(a, to, st);
+        return launch_route_as<MODE, 16, 16>(a, to, st);
     }
+    if (a.experts <= 256) return launch_route_as<MODE, 64, 4>(a, to, st);
+    if (a.experts <= 512) return launch_route_as<MODE, 64, 8>(a, to, st);
+    if (a.experts <= 1024) return launch_route_as<MODE, 64, 16>(a, to, st);
+    return launch_route_as<MODE == kSifted ? kByValue : MODE, 64, 0>(a, to, st);
 }
 
 // Arguments of a sort; EIF_HIP_OK where it may be launched.
@@ -791,24 +860,6 @@ int check_sort(int tokens, int top, int experts, const int32_t *offsets, const i
     if (tokens > 0 && (!row || !slot)) return EIF_HIP_E_ARG;
     const size_t need = eif_hip_moe_sort_bytes(tokens, top, experts);
     return need > 0 && (!work || work_bytes < need) ? EIF_HIP_E_ARG : EIF_HIP_OK;
-}
-
-int launch_sort(const int32_t *ids, int tokens, int top, int experts, int32_t *offsets, int32_t *row, int32_t *slot, void *work,
-                hipStream_t st)
-{
-    const int pairs = tokens * top, blocks = sort_blocks(pairs), share = blocks > 1 ? sort_share(pairs) : pairs;
-    int bits = 0;
-    while (1 << bits < experts) ++bits;
-    int32_t *counts = static_cast<int32_t *>(work);
-    if (blocks > 1) {
-        sort_count_kernel<<<blocks, 1024, experts * sizeof(int32_t), st>>>(ids, pairs, share, experts, counts);
-        EIF_HIP_LAUNCHED();
-    }
-    const int waves = sort_waves(experts, share);
-    const size_t lds = ((size_t)(waves + 2) * experts + 16) * sizeof(int32_t);
-    sort_place_kernel<<<blocks, 64 * waves, lds, st>>>(ids, pairs, share, experts, bits, top, counts, blocks, offsets, row, slot);
-    EIF_HIP_LAUNCHED();
-    return EIF_HIP_OK;
 }
 
 template <typename T>
@@ -862,6 +913,7 @@ int eif_hip_moe_route(const void *logits, int type, int64_t ldl, int tokens, con
     if (tokens > 0 && (!logits || !ids || !weights)) return EIF_HIP_E_ARG;
     if (!aligned(logits, type == EIF_HIP_F32 ? 4 : 2) || !aligned(ids, 4) || !aligned(weights, 4)) return EIF_HIP_E_ARG;
     hipStream_t st = (hipStream_t)stream;
+    const SortedTo to{offsets, row, slot, work};
     if (tokens > 0) {
         RouteArgs a{};
         a.logits = logits, a.bias = s.bias, a.ids = ids, a.weights = weights, a.ldl = ldl, a.type = type, a.tokens = tokens;
@@ -870,10 +922,10 @@ int eif_hip_moe_route(const void *logits, int type, int64_t ldl, int tokens, con
         a.group_size = s.experts / s.groups;
         a.group_magic = (uint32_t)((0xffffffffull + a.group_size) / a.group_size);
         const bool by_value = s.bias || (a.groups > 1 && a.best == 2), sifted = s.bias && s.score == EIF_HIP_SCORE_SIGMOID;
-        const int rc = sifted ? launch_route<kSifted>(a, st) : by_value ? launch_route<kByValue>(a, st) : launch_route<kByLogit>(a, st);
-        if (rc) return rc;
+        if (sifted) return launch_route<kSifted>(a, to, st);
+        return by_value ? launch_route<kByValue>(a, to, st) : launch_route<kByLogit>(a, to, st);
     }
-    return sorted ? launch_sort(ids, tokens, s.top_k, s.experts, offsets, row, slot, work, st) : EIF_HIP_OK;
+    return sorted ? launch_sort(ids, 0, s.top_k, s.experts, to, st) : EIF_HIP_OK;
 }
 
 int eif_hip_moe_sort(const int32_t *ids, int tokens, int top_k, int experts, int32_t *offsets, int32_t *row, int32_t *slot, void *work,
@@ -882,7 +934,7 @@ int eif_hip_moe_sort(const int32_t *ids, int tokens, int top_k, int experts, int
     const int rc = check_sort(tokens, top_k, experts, offsets, row, slot, work, work_bytes);
     if (rc) return rc;
     if ((tokens > 0 && !ids) || !aligned(ids, 4)) return EIF_HIP_E_ARG;
-    return launch_sort(ids, tokens, top_k, experts, offsets, row, slot, work, (hipStream_t)stream);
+    return launch_sort(ids, tokens, top_k, experts, SortedTo{offsets, row, slot, work}, (hipStream_t)stream);
 }
 
 int eif_hip_moe_combine(const float *y, int64_t ldy, int rows, const int32_t *slot, const float *weights, int tokens, int top_k,
