@@ -236,22 +236,6 @@ __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
     if (n < a.rows) *y = base + out;
 }
 
-// W x, 16 ranks by 16 tokens by 32 columns, on a lane's 8 columns of each. Of one 16-bit type: one instruction, whose products are
-// exact; else as FP32, four columns at a time.
-template <typename X, typename W>
-EIF_DEV v4f product32(const Pack<W, 8> &w, const Pack<X, 8> &x, v4f acc)
-{
-    if constexpr (std::is_same<X, W>::value && std::is_same<X, __hip_bfloat16>::value) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), acc, 0, 0, 0);
-    } else if constexpr (std::is_same<X, W>::value && std::is_same<X, __half>::value) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), acc, 0, 0, 0);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w.v[j]), to_f32(x.v[j]), acc, 0, 0, 0);
-        return acc;
-    }
-}
-
 // A float as the sum of three bf16, exactly (8 bits of its 24 each), four at a time; an infinity or NaN is in the first alone.
 EIF_DEV void planes4(v4f v, uint2 *p)
 {
@@ -266,6 +250,22 @@ EIF_DEV void planes4(v4f v, uint2 *p)
 #pragma unroll
     for (int i = 0; i < 3; ++i)
         p[i] = make_uint2(__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302));
+}
+
+// W x, 16 ranks by 16 tokens by 32 columns, on a lane's 8 columns of each. Of one 16-bit type: one instruction, whose products are
+// exact; else as FP32, four columns at a time.
+template <typename X, typename W>
+EIF_DEV v4f product32(const Pack<W, 8> &w, const Pack<X, 8> &x, v4f acc)
+{
+    if constexpr (std::is_same<X, W>::value && std::is_same<X, __hip_bfloat16>::value) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), acc, 0, 0, 0);
+    } else if constexpr (std::is_same<X, W>::value && std::is_same<X, __half>::value) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w.v[j]), to_f32(x.v[j]), acc, 0, 0, 0);
+        return acc;
+    }
 }
 
 // Many rows: a workgroup of 8 waves has TT tiles of 16 rows and a share of their outputs. First V = A x of the rows, for all the
@@ -357,10 +357,27 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
 #pragma unroll
                 for (int u = 0; u < DX; ++u) {
                     if (cb + u < c1) {
+                        if constexpr (planes && sizeof(X) == 4) {
+                            // x as planes too: 256 rows of 64 ranks 33 us, with FP32 instructions 51; of 16 ranks as long either way
 #pragma unroll
-                        for (int r = 0; r < RN; ++r) {
+                            for (int t = 0; t < TT; ++t) {
+                                uint2 lo[3], hi[3];
+                                planes4(v4f{xr[u][t].v[0], xr[u][t].v[1], xr[u][t].v[2], xr[u][t].v[3]}, lo);
+                                planes4(v4f{xr[u][t].v[4], xr[u][t].v[5], xr[u][t].v[6], xr[u][t].v[7]}, hi);
 #pragma unroll
-                            for (int t = 0; t < TT; ++t) acc[r][t] = product32(w[u % DW][r], xr[u][t], acc[r][t]);
+                                for (int i = 2; i >= 0; --i) {
+                                    const v8bf p = __builtin_bit_cast(v8bf, make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y));
+#pragma unroll
+                                    for (int r = 0; r < RN; ++r)
+                                        acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w[u % DW][r]), p, acc[r][t], 0, 0, 0);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < RN; ++r) {
+#pragma unroll
+                                for (int t = 0; t < TT; ++t) acc[r][t] = product32(w[u % DW][r], xr[u][t], acc[r][t]);
+                            }
                         }
                         load_x(xr[u], cb + u + DX);
                         load_w(w[u % DW], cb + u + DW);
@@ -581,8 +598,9 @@ template <typename X, typename W, bool VEC, int TT>
 int launch_tiles_as(AdapterArgs a, int workgroups, hipStream_t st)
 {
     const int tiles = eif_ceil_div(a.M, 16 * TT);
-    a.splits = std::max(1, std::min(eif_ceil_div(a.rows, 128), workgroups / tiles));
     a.tiles_xcd = eif_ceil_div(tiles, 8);
+    // workgroups that run at once: one more would begin when the others end (600 rows through 2560x2560 26.8 us with 520, 19.9 with 480)
+    a.splits = std::max(1, std::min(eif_ceil_div(a.rows, 128), workgroups / (a.tiles_xcd * 8)));
     adapter_tile_kernel<X, W, VEC, TT><<<(unsigned)(a.tiles_xcd * 8 * a.splits), 512, 0, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
@@ -598,7 +616,7 @@ template <typename X, typename W>
 int launch_adapters_as(AdapterArgs a, hipStream_t st)
 {
     const bool vec = aligned(a.x, 16) && a.ldx % 8 == 0 && a.cols % 8 == 0;
-    if (a.M <= 64) {
+    if (a.M * std::min(a.rank_tiles, 2) <= 512) {
         a.splits = eif_ceil_div(a.rows, 1024);
         const unsigned blocks = (unsigned)(eif_ceil_div(a.M, 8) * 8 * a.splits);
         if (a.rank_tiles == 1)
