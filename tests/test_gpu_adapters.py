@@ -127,6 +127,32 @@ def test_not_finite(gpu, m, types):
     assert (np.abs(got[rest] - want[rest]) <= tol[rest]).all()
 
 
+@pytest.mark.parametrize("m", [20, 600, 4200])
+@pytest.mark.parametrize("types", [("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")])
+def test_broken_adapter(gpu, m, types):
+    """Matrices with infinities and NaN in one slot do not reach the rows of other slots, or of none."""
+    import torch
+    rows, cols = 70, 130
+    c = Case(gpu, 4, 4, rows, cols, 20, types[1])
+    rng = np.random.default_rng(m)
+    dt = torch.from_numpy(c.pairs[1][0]).to(getattr(torch, {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}[types[1]])).dtype
+    a, b = torch.randn(20, cols).to(dt), torch.randn(rows, 20).to(dt)
+    a[3, 5], a[17, 100], b[9, 2], b[50, 19] = float("inf"), float("nan"), float("-inf"), float("nan")
+    c.h.set(1, a.cuda(), b.cuda(), 1.0)
+    x, slot = mx4_ref.activations(rng, m, cols), slots_of(rng, m, 4, "any")
+    slot[:4] = [0, 1, 2, -1]
+    x = dev(x, types[0])
+    base = rng.standard_normal((m, rows)).astype(np.float32)
+    y = torch.empty((m, rows), device="cuda")
+    c.h.linear(x, dev(slot), y, dev(base))
+    torch.cuda.synchronize()
+    pairs = {s: p for s, p in c.pairs.items() if s != 1}
+    rest = slot != 1
+    want, tol = moe_ref.adapters(host(x), slot, pairs, base, rows)
+    got = host(y)
+    assert (np.abs(got[rest] - want[rest]) <= tol[rest]).all() and np.isnan(got[~rest]).any(1).all()
+
+
 def test_slots_are_replaced(gpu):
     """A slot takes another adapter, of another rank, and none; the others stay."""
     import torch

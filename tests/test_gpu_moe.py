@@ -104,6 +104,9 @@ ROUTE = [  # tokens, experts, top, groups, kept, best
     (18, 512, 22, 64, 9, 1), (10, 1000, 33, 10, 3, 2), (9, 1024, 64, 1, 1, 1), (12, 1025, 3, 5, 4, 2), (10, 4096, 64, 64, 16, 2),
     (9, 4095, 5, 63, 2, 1), (27, 64, 8, 64, 12, 2), (1030, 64, 8, 1, 1, 1), (1100, 256, 16, 8, 4, 2), (1500, 96, 5, 4, 2, 1),
     (1025, 30, 3, 1, 1, 1), (1024, 16, 16, 16, 5, 2), (2000, 128, 8, 16, 4, 2), (1027, 7, 4, 7, 4, 1),
+    # where the lanes of a token change, and where the sort is in the same launch
+    (64, 64, 8, 1, 1, 1), (65, 64, 8, 8, 4, 2), (8, 200, 6, 8, 4, 2), (9, 256, 8, 1, 1, 1), (2049, 256, 8, 8, 4, 2), (2050, 100, 16, 5, 3, 1),
+    (4100, 200, 7, 1, 1, 1), (2048, 66, 5, 6, 3, 2),
 ]
 
 
@@ -151,9 +154,9 @@ def test_route_far_offsets(gpu):
     torch.cuda.empty_cache()
 
 
-def test_scores_near_one(gpu):
+@pytest.mark.parametrize("experts", [64, 256, 1000])
+def test_scores_near_one(gpu, experts):
     """Scores that 32 bits cannot tell apart: the logits' order without a bias, the 64-bit sums' with one."""
-    experts = 64
     l = np.zeros((4, experts), np.float32)
     l[0] = 20.0 + np.arange(experts) * 2.0 ** -10           # sigmoid: 1 - 2e-9 and less
     l[1] = 20.0 - np.arange(experts) * 2.0 ** -10
@@ -163,6 +166,18 @@ def test_scores_near_one(gpu):
         for score in (moe_ref.SIGMOID, moe_ref.SOFTMAX):
             check_route(gpu, dev(l), 8, score=score, bias=bias)
             check_route(gpu, dev(l), 8, score=score, bias=bias, groups=8, groups_kept=2, group_best=2)
+
+
+def test_many_equals(gpu):
+    """More equals than there is room for: the lowest indices, of experts and of groups."""
+    for tokens, experts in ((3, 64), (5, 256), (2100, 256), (3, 700)):
+        x = np.zeros((tokens, experts), np.float32)
+        x[1] = np.where(np.arange(experts) % 3 == 1, 0.5, -0.25)
+        x[2, experts // 2:] = 1.0
+        for score in (moe_ref.SOFTMAX, moe_ref.SIGMOID):
+            for bias in (None, np.zeros(experts, np.float32), np.where(np.arange(experts) % 2, 0.25, 0.0).astype(np.float32)):
+                check_route(gpu, dev(x), 16, score=score, bias=bias)
+                check_route(gpu, dev(x), 7, score=score, bias=bias, groups=4, groups_kept=2, group_best=2, renormalise=False)
 
 
 SORT = [(0, 4, 7), (1, 1, 1), (1, 3, 2), (33, 2, 8), (100, 7, 300), (1024, 8, 64), (1023, 8, 513), (1025, 8, 1024), (2500, 3, 1025), (7, 4096, 9),

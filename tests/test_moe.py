@@ -120,6 +120,25 @@ def test_combine_refuses(fake):  # noqa: F811
     """)
 
 
+@pytest.mark.parametrize("tokens,experts,top,bias,launches,grid,block", [
+    (1, 32, 4, False, 1, 1, 64), (64, 64, 8, False, 1, 1, 1024), (65, 64, 8, False, 2, 17, 64), (8, 256, 8, True, 1, 1, 512),
+    (9, 256, 8, True, 2, 9, 64), (2048, 256, 8, True, 3, 2048, 64), (2049, 256, 8, True, 3, 513, 64), (16001, 256, 8, True, 3, 1001, 256),
+    (3, 4096, 8, False, 2, 3, 64), (5000, 4096, 64, True, 3, 5000, 64), (600, 1024, 17, False, 3, 600, 64), (4096, 64, 1, False, 2, 1024, 64),
+])
+def test_route_launches(fake, tokens, experts, top, bias, launches, grid, block):  # noqa: F811
+    """A few tokens are chosen and sorted in one launch; up to 4096 pairs are sorted in one, more in two."""
+    run(fake, CALLS + f"""
+    tokens, experts, top = {tokens}, {experts}, {top}
+    need = lib.eif_hip_moe_sort_bytes(tokens, top, experts)
+    assert route(tokens=tokens, experts=experts, ldl=experts, top_k=top, bias=X.value if {bias} else None, score=1, offsets=X, row=X, slot=X,
+                 work=X, bytes=need) == 0
+    assert fake.fake_launches() == {launches} and (fake.fake_launch_grid(0), fake.fake_launch_block(0)) == ({grid}, {block})
+    assert (need > 0) == (tokens * top > 4096)
+    assert route(tokens=tokens, experts=experts, ldl=experts, top_k=top, bias=X.value if {bias} else None, score=1) == 0
+    assert fake.fake_launches() == 1
+    """)
+
+
 ADAPTERS = """
     ARG, LIMIT, NOMEM, DEVICE = -1, -4, -3, -2
     at = lambda n: vp(X.value + n)
@@ -197,6 +216,21 @@ def test_adapters_linear_refuses(fake):  # noqa: F811
     fake.fake_device(0)
     fake.fake_reset(); fake.fake_fail_launch(0)
     assert lib.eif_hip_adapters_linear(h, X, 0, 96, X, None, 0, X, 64, 5, None) == DEVICE
+    lib.eif_hip_adapters_destroy(h)
+    """)
+
+
+@pytest.mark.parametrize("M,rank,block,grid", [
+    (1, 16, 1024, 8), (9, 16, 1024, 16), (512, 16, 1024, 512), (513, 16, 512, 40 * 1), (256, 64, 1024, 256), (257, 64, 512, 24), (4095, 16, 512, 256),
+    (4096, 16, 512, 128), (1 << 24, 16, 512, 1 << 19),
+])
+def test_adapters_forms(fake, M, rank, block, grid):  # noqa: F811
+    """A row a workgroup up to 512 rows of up to 16 ranks, or 256; then tiles of 16 rows, from 4096 rows on of 32."""
+    run(fake, ADAPTERS + f"""
+    rc, h = create(rank={rank})
+    fake.fake_reset()
+    assert rc == 0 and lib.eif_hip_adapters_linear(h, X, 0, 96, X, None, 0, X, 64, {M}, None) == 0
+    assert fake.fake_launches() == 1 and (fake.fake_launch_grid(0), fake.fake_launch_block(0)) == ({grid}, {block})
     lib.eif_hip_adapters_destroy(h)
     """)
 
