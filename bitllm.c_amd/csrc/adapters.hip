@@ -106,6 +106,8 @@ EIF_DEV void by_tiles(int n, F f)
 // same row repeat (out of the XCD's L2, where they all run), and from it its outputs: one launch instead of two with the sums of the
 // first in memory between them. What a CU reads through its L1 bounds it (64 bytes a clock), so that x, which 16 lanes share, comes
 // from LDS. ONE: ranks up to 16, whose matrices are read before the rank is known (what lies behind it is zeros).
+// One row of 16 ranks through 2560x2560 3.8 us, of which 1.7 are an empty launch's and the rest a chain of slot, A and sums; 48 rows of 48
+// requests with 8 to 64 ranks through 4096x4096 11.5 us (each of a row's four workgroups reads its A, up to 512 KB).
 template <typename X, typename W, bool VEC, bool ONE>
 __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
 {
@@ -273,7 +275,9 @@ EIF_DEV v4f product32(const Pack<W, 8> &w, const Pack<X, 8> &x, v4f acc)
 // sums meet in LDS, where each row keeps those of its own adapter. Then base + B V, two tiles of 16 outputs at a time, with every adapter in
 // turn, each row taking its own one's. The tokens are the columns of both products. bf16 B: V as three bf16 planes on 16x16x32
 // instructions, whose products are exact, a sixteenth of the time of FP32 ones; else FP32 instructions. Loads run ahead: x and A two or
-// four steps, base and B two or three.
+// four steps, base and B two or three. 8192 bf16 rows of 64 ranks through 4096x4096 88 us where they share an adapter (3.8 TB/s: 25 us the
+// first product with its launch, 66 the second, copying base to y 58), 114 where nine requests meet in tiles, whose workgroups go
+// through x and the outputs for two adapters and end last. 1531 FP32 rows of 16 ranks through 6912x2560 32 us (3.1 TB/s).
 template <typename X, typename W, bool VEC, int TT>
 __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(AdapterArgs a)
 {
@@ -611,6 +615,8 @@ int launch_tiles_as(AdapterArgs a, int workgroups, hipStream_t st)
     return EIF_HIP_OK;
 }
 
+// Tiles of 32 rows read A and B half as often, and leave half as many workgroups: 4096 rows of 16 ranks through 4096x4096 55 us with them,
+// 59 with tiles of 16, 8192 of 64 88 and 105; 3000 77 either way; 1531 rows of five requests through 6912x2560 51 and 48.
 template <typename X, typename W, bool VEC>
 int launch_tiles(const AdapterArgs &a, hipStream_t st)
 {
@@ -621,6 +627,9 @@ template <typename X, typename W>
 int launch_adapters_as(AdapterArgs a, hipStream_t st)
 {
     const bool vec = aligned(a.x, 16) && a.ldx % 8 == 0 && a.cols % 8 == 0;
+    // A row a workgroup does not care which adapters meet, a tile does (us, rows of one adapter / of 32 in any order; 512 rows of 16 ranks
+    // through 2560x2560: rows 21 / 22, tiles 18 / 88; 256 of 64 through 4096x4096 42 / 49, 33 / 397; 512 81 / 94, 35 / 427; 64 12 / 16, 29 /
+    // 296): up to the sizes of a batch of single tokens the rows.
     if (a.M * std::min(a.rank_tiles, 2) <= 512) {
         a.splits = eif_ceil_div(a.rows, 1024);
         const unsigned blocks = (unsigned)(eif_ceil_div(a.M, 8) * 8 * a.splits);

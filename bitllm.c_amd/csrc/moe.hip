@@ -322,7 +322,10 @@ EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val,
 //   The choice: the top-th largest of the lanes' largest is at most the top-th largest of all, so that the experts at or above it hold the
 // chosen ones, and are few more. They go to LDS, and each counts those that come before it. Sifted: the candidates are those within
 // the error of 32 bits, and only they are computed in 64, an expert a lane in place of all, or the groups where two of them are nearer to
-// each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly. The instructions bound it.
+// each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly.
+//   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 14 us, 20 where two
+// groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits, where reading
+// them takes 3.3. A few tokens are one wave's chain: 64 tokens 6.1 us.
 template <int MODE, int LPT, int VPL>
 EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, char *lds)
 {
@@ -604,6 +607,7 @@ EIF_DEV uint64_t same_id(int id, bool live, int bits)
 
 // A workgroup places the pairs [blockIdx share, + share): a pair's place is the pairs of lower experts, those of its expert in
 // workgroups, waves and steps before, and in the lanes before. Each wave has a run of the pairs in order, and counters of its own.
+// 262144 pairs of 128 experts 8.0 us behind 2.4 of counting, 66 of 8 2.8 us alone: a chain of barriers, loads and LDS, not of bytes.
 // cnt: [waves][experts], then the sums [experts], those of workgroups before [experts], and of the waves [16].
 EIF_DEV void sort_place(const int32_t *ids, int pairs, int share, int experts, int bits, int top, const int32_t *counts, int blocks,
                         int32_t *offsets, int32_t *row, int32_t *slot, int32_t *cnt)
