@@ -220,7 +220,10 @@ EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
         if (g < a.groups && j == 0) {
             const bool both = a.best == 2 && b2 > none;
             worth[g] = both ? b1 + b2 : b1;
-            if constexpr (SIFTED) worth[a.groups + g] = sift_error(b1) + (both ? sift_error(b2) + fabsf(b1 + b2) * 0x1.02p-24f : 0.0f);
+            if constexpr (SIFTED) {   // of a group that is shut out: none
+                const float off = sift_error(b1) + (both ? sift_error(b2) + fabsf(b1 + b2) * 0x1.02p-24f : 0.0f);
+                worth[a.groups + g] = b1 > none ? off : 0.0f;
+            }
         }
     }
     wave_lds_order();
@@ -323,7 +326,7 @@ EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val,
 // chosen ones, and are few more. They go to LDS, and each counts those that come before it. Sifted: the candidates are those within
 // the error of 32 bits, and only they are computed in 64, an expert a lane in place of all, or the groups where two of them are nearer to
 // each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly.
-//   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 14 us, 20 where two
+//   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 15 us, 18 where two
 // groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits, where reading
 // them takes 3.3. A few tokens are one wave's chain: 64 tokens 6.1 us.
 template <int MODE, int LPT, int VPL>
@@ -429,8 +432,16 @@ EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane,
             if constexpr (MODE == kSifted) {
                 if (__ballot(!sure)) {   // 64 bits tell
                     double *value = reinterpret_cast<double *>(lds);
-#pragma unroll 4
-                    for (int e = sub; e < a.experts; e += LPT) value[e] = value_of(a, logit_at(a, row + e), e, 0.0, 1.0);
+                    float b[kEach];
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) b[i] = a.bias[min(i * LPT + sub, a.experts - 1)];
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) {
+                        const int e = i * LPT + sub;
+                        const double v = sigmoid64(l[i]) + (double)b[i];
+                        if (e < a.experts) value[e] = l[i] > -INFINITY && b[i] > none ? v : -INFINITY;
+                        __builtin_amdgcn_sched_barrier(0);   // one after the other, for the registers' sake
+                    }
                     keep = kept_groups<LPT, false>(a, lane, value, sure);
                 }
             }

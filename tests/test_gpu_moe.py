@@ -162,10 +162,19 @@ def test_scores_near_one(gpu, experts):
     l[1] = 20.0 - np.arange(experts) * 2.0 ** -10
     l[2] = np.float32(1.0) + np.arange(experts) * np.float32(2.0 ** -23)
     l[3] = np.float32(1.0) - np.arange(experts) * np.float32(2.0 ** -24)
-    for bias in (None, np.zeros(experts, np.float32), np.full(experts, -1.0, np.float32), np.full(experts, 100.0, np.float32)):
+    l = np.concatenate([l, logits_of(np.random.default_rng(4), 5, experts, "plain")])
+    shut = np.zeros(experts, np.float32)   # whole groups that are shut out beside near ones
+    shut[:experts // 8] = -np.inf
+    most = np.full(experts, -np.inf, np.float32)
+    most[experts // 8 * 3:experts // 8 * 4] = 0.0
+    large = (np.random.default_rng(3).integers(-3, 4, experts) * 2.0 ** 20).astype(np.float32)   # 32 bits keep an eighth of a score's range
+    for bias in (None, np.zeros(experts, np.float32), np.full(experts, -1.0, np.float32), np.full(experts, 100.0, np.float32), shut, most,
+                 large, np.full(experts, 1e6, np.float32)):
         for score in (moe_ref.SIGMOID, moe_ref.SOFTMAX):
             check_route(gpu, dev(l), 8, score=score, bias=bias)
-            check_route(gpu, dev(l), 8, score=score, bias=bias, groups=8, groups_kept=2, group_best=2)
+            for kept in (2, 7):
+                check_route(gpu, dev(l), 8, score=score, bias=bias, groups=8, groups_kept=kept, group_best=2)
+                check_route(gpu, dev(l), 8, score=score, bias=bias, groups=8, groups_kept=kept, group_best=1, renormalise=False)
 
 
 def test_many_equals(gpu):
