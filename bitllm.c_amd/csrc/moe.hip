@@ -756,19 +756,30 @@ struct CombineArgs {
     int cols, chunks, log_cols;   // threads of a token in a workgroup (2^log_cols of them), and workgroups of a token's columns
 };
 
-// A thread has V adjacent columns of a token. Bound by memory: 2048 tokens of 8 rows of 2048 with a residual, to bf16, 31.4 us, 5.0 TB/s of
-// what it reads and writes, which is what a large copy reaches (34 us a row after the other in place of four at a time; a few tokens
-// 3.1 in place of 3.5).
-template <typename T, int V>
+// A thread has four adjacent columns of a token (of the row's last ones fewer), 16 bytes at a time: rows that are not ALIGNED to them
+// too, which loads of 16 bytes at any float and stores at any element serve (2000 tokens of 8 rows of 2047 32.7 us, with a
+// column a thread 45.7). Bound by memory: 2048 tokens of 8 rows of 2048 with a residual, to bf16, 31.4 us, 5.0 TB/s of what it reads
+// and writes, which is what a large copy reaches (34 us a row after the other in place of four at a time; a few tokens 3.1 in place of
+// 3.5).
+template <typename T, bool ALIGNED>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 {
+    struct alignas(ALIGNED ? 16 : 4) In { float v[4]; };
+    struct alignas(ALIGNED ? 4 * sizeof(T) : sizeof(T)) Out { T v[4]; };
     const int64_t block = blockIdx.x / a.chunks;
     const int64_t t = (block << (8 - a.log_cols)) + (threadIdx.x >> a.log_cols);
-    const int c = V * ((int)(blockIdx.x - block * a.chunks) * 256 + (int)(threadIdx.x & (a.cols - 1)));
+    const int c = 4 * ((int)(blockIdx.x - block * a.chunks) * 256 + (int)(threadIdx.x & (a.cols - 1)));
     if (t >= a.tokens || c >= a.dim) return;
-    float acc[V];
+    const int n = ALIGNED ? 4 : min(a.dim - c, 4);
+    const auto load = [&](const float *y) {
+        if (n == 4) return *reinterpret_cast<const In *>(y);
+        In r{};
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+        for (int i = 0; i < 3; ++i)
+            if (i < n) r.v[i] = y[i];
+        return r;
+    };
+    float acc[4] = {};
     const int32_t *slot = a.slot + t * a.top;
     for (int k0 = 0; k0 < a.top; k0 += 4) {   // four rows under way
         int s[4];
@@ -780,36 +791,34 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
             w[k] = a.weights ? a.weights[t * a.top + at] : 1.0f;
             if (k0 + k >= a.top) s[k] = -1;
         }
-        float v[4][V];
+        In v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const bool there = (unsigned)s[k] < (unsigned)a.rows;
-            const float *y = a.y + (there ? s[k] : 0) * a.ldy + c;
-            if (there) {
-                if constexpr (V == 4) *reinterpret_cast<float4 *>(v[k]) = *reinterpret_cast<const float4 *>(y);
-                else v[k][0] = y[0];
-            }
-        }
+        for (int k = 0; k < 4; ++k)
+            if ((unsigned)s[k] < (unsigned)a.rows) v[k] = load(a.y + s[k] * a.ldy + c);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if ((unsigned)s[k] < (unsigned)a.rows) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = fmaf(w[k], v[k][i], acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = fmaf(w[k], v[k].v[i], acc[i]);
             }
         }
     }
     if (a.add) {
-        const float *y = a.add + t * a.lda + c;
-        float v[V];
-        if constexpr (V == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(y);
-        else v[0] = y[0];
+        const In v = load(a.add + t * a.lda + c);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += v[i];
+        for (int i = 0; i < 4; ++i) acc[i] += v.v[i];
     }
-    struct alignas(V * sizeof(T)) Out { T v[V]; } o;
+    Out o;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(acc[i]);
-    *reinterpret_cast<Out *>(static_cast<T *>(a.out) + t * a.ldo + c) = o;
+    for (int i = 0; i < 4; ++i) o.v[i] = from_f32<T>(acc[i]);
+    T *out = static_cast<T *>(a.out) + t * a.ldo + c;
+    if (n == 4) {
+        *reinterpret_cast<Out *>(out) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) out[i] = o.v[i];
+    }
 }
 
 // ---- launches ----
@@ -900,18 +909,18 @@ int check_sort(int tokens, int top, int experts, const int32_t *offsets, const i
 template <typename T>
 int launch_combine(CombineArgs a, hipStream_t st)
 {
-    const bool vec = a.dim % 4 == 0 && aligned(a.y, 16) && a.ldy % 4 == 0 && (!a.add || (aligned(a.add, 16) && a.lda % 4 == 0)) &&
+    const bool whole = a.dim % 4 == 0 && aligned(a.y, 16) && a.ldy % 4 == 0 && (!a.add || (aligned(a.add, 16) && a.lda % 4 == 0)) &&
                      aligned(a.out, 4 * sizeof(T)) && a.ldo % 4 == 0;
-    const int units = vec ? a.dim / 4 : a.dim;   // threads that a token's columns take
+    const int units = eif_ceil_div(a.dim, 4);   // threads that a token's columns take
     a.log_cols = 0;
     while (a.log_cols < 8 && 1 << a.log_cols < units) ++a.log_cols;
     a.cols = 1 << a.log_cols;
     a.chunks = eif_ceil_div(units, 256);
     const int64_t blocks = ((int64_t)a.tokens + (256 >> a.log_cols) - 1) / (256 >> a.log_cols) * a.chunks;
-    if (vec)
-        combine_kernel<T, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+    if (whole)
+        combine_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(a);
     else
-        combine_kernel<T, 1><<<(unsigned)blocks, 256, 0, st>>>(a);
+        combine_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
