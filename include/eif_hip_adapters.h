@@ -43,6 +43,8 @@ int eif_hip_adapters_info(const eif_hip_adapters *a, int *slots, int *rows, int 
  *   slot [M] int32: rows in any order of slots; a row whose slot is empty or outside of [0, slots) gets base[m].
  *   base [M, ldbase] FP32, e.g. the projection's output; it may be y itself (ldbase == ldy), or NULL (0).
  *   y [M, ldy] FP32.
+ * The form goes by M and max_rank, since the host does not see the slots: up to 512 rows (256 where max_rank is more than 16) each row is
+ * worked on by itself; of more rows those that share an adapter should lie together.
  * Products and sums in FP32, in an order that M and the shapes set, not the slots of other rows. One launch; nothing is allocated and
  * nothing kept, so that any number of calls may run at once and be captured into graphs. M up to 2^24, else EIF_HIP_E_LIMIT. */
 int eif_hip_adapters_linear(const eif_hip_adapters *a, const void *x, int type, int64_t ldx, const int32_t *slot, const float *base,
