@@ -184,7 +184,8 @@ __host__ __device__ constexpr int route_lds(int experts, int groups)
 EIF_DEV float sift_error(float v) { return fmaf(fabsf(v), 0x1.02p-24f, 0x1p-22f); }
 
 // The groups whose experts may be chosen, a bit each, from what the experts are worth (val [experts], behind them room for the groups).
-// SIFTED: `sure` says whether the kept ones are worth more than the others beyond any error.
+// SIFTED: `sure` says whether the kept ones are worth more than the others beyond any error. It is not known of a group whose sum leaves
+// 32 bits, as that of two biases of the lowest value does.
 template <int LPT, bool SIFTED, typename KEY>
 EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
 {
@@ -229,6 +230,7 @@ EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
     wave_lds_order();
     uint64_t keep = 0;
     KEY kept_least = INFINITY, dropped_most = none;
+    bool known = true;
     for (int g0 = 0; g0 < a.groups; g0 += LPT) {
         const int g = g0 + sub;
         int better = a.kept;
@@ -238,7 +240,8 @@ EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
 #pragma unroll 4
             for (int h = 0; h < a.groups; ++h) better += worth[h] > w || (worth[h] == w && h < g);
             if constexpr (SIFTED) {
-                const float off = worth[a.groups + g];
+                const float off = worth[a.groups + g];   // finite only where what it is worth is, and 0 of a group that is shut out
+                known = known && off < INFINITY;
                 if (better < a.kept) kept_least = fminf(kept_least, w - off);
                 else dropped_most = larger(dropped_most, w + off);
             }
@@ -248,7 +251,7 @@ EIF_DEV uint64_t kept_groups(const RouteArgs &a, int lane, KEY *val, bool &sure)
     }
     if constexpr (SIFTED) {
         const float least = -lanes_max<LPT>(-kept_least), most = lanes_max<LPT>(dropped_most);
-        sure = least > most || !(most > none);
+        sure = known && (least > most || !(most > none));
     }
     wave_lds_order();
     return keep;

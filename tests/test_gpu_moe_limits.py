@@ -1,0 +1,64 @@
+"""Routing to experts on the GPU (include/eif_hip_moe.h) at the ends of what scores and biases hold, against the definition in 64
+bits: sums of biases that 32 bits do not hold."""
+import numpy as np
+import pytest
+
+import moe_ref
+from test_gpu_moe import dev, host, ints
+
+pytestmark = pytest.mark.gpu
+
+LOWEST, MOST = np.finfo(np.float32).min, np.finfo(np.float32).max
+
+
+def check(gpu, rows, tokens, top, type="f32", sorted_too=False, **spec):
+    """Logits `rows`, repeated to so many tokens. A weight is computed in 64 bits and rounded once: off by 2^-24 of it, or 2^-150, and by
+    some 1e-14 of it before."""
+    import torch
+    few = dev(rows, type)
+    at = np.arange(tokens) % rows.shape[0]
+    x = few[torch.from_numpy(at).cuda()].contiguous()
+    ids, w = ints(tokens * top).view(tokens, top), torch.full((tokens, top), float("nan"), device="cuda")
+    places = {}
+    if sorted_too:
+        need = gpu.moe_sort_bytes(tokens, top, rows.shape[1])
+        places = dict(offsets=ints(rows.shape[1] + 1), row=ints(tokens * top), slot=ints(tokens * top),
+                      work=torch.full((need,), 0x5A, dtype=torch.uint8, device="cuda") if need else None)
+    b = spec.get("bias")
+    gpu.moe_route(x, ids, w, **{**spec, "bias": None if b is None else dev(b)}, **places)
+    torch.cuda.synchronize()
+    want_ids, want = moe_ref.route(host(few), top, **spec)
+    want_ids, want = want_ids[at], want[at]
+    got = host(ids)
+    bad = np.nonzero((got != want_ids).any(1))[0]
+    assert not bad.size, (spec, bad[:5], got[bad[:3]].tolist(), want_ids[bad[:3]].tolist())
+    gw = host(w).astype(np.float64)
+    off = np.abs(gw - want) / (1.01 * 2.0 ** -24 * np.abs(want) + 2.0 ** -149)
+    assert (off <= 1.0).all(), (spec, np.max(off))
+    if sorted_too:
+        for p, v, name in zip((places["offsets"], places["row"], places["slot"]), moe_ref.sort(want_ids, rows.shape[1]), ("offsets", "row", "slot")):
+            assert np.array_equal(host(p), v), name
+
+
+@pytest.mark.parametrize("tokens,experts,groups", [(3, 16, 4), (5, 64, 32), (7, 64, 64), (7, 256, 8), (7, 256, 64), (2100, 256, 8), (2100, 256, 64),
+                                                   (4100, 96, 48), (5, 1000, 10), (3, 1100, 11)])
+def test_groups_of_lowest_biases(gpu, tokens, experts, groups):
+    """Two biases whose sum 32 bits do not hold: a group of them is worth more than one that is shut out, and as much as 64 bits say."""
+    rng = np.random.default_rng(experts + groups)
+    rows = (1.5 * rng.standard_normal((7, experts))).astype(np.float32)
+    size = experts // groups
+    rows[0, :size] = -np.inf
+    rows[1, rng.random(experts) < 0.5] = -np.inf
+    rows[2, size:] = -np.inf
+    group = np.arange(experts) // size
+    worths = np.array([LOWEST, LOWEST / 2, MOST, MOST * 0.75, -np.inf, np.nan, np.inf, 0.1], np.float32)
+    biases = [np.full(experts, LOWEST, np.float32), np.where(group == groups - 1, 0.25, LOWEST).astype(np.float32),
+              np.where(group % 2, -np.inf, LOWEST).astype(np.float32), np.where(group % 2, MOST, np.inf).astype(np.float32)]
+    biases += [worths[rng.integers(8, size=groups)][group] for _ in range(6)]
+    biases += [worths[rng.integers(8, size=experts)] for _ in range(2)]
+    biases += [np.where(rng.random(experts) < 0.7, LOWEST, (0.2 * rng.standard_normal(experts)).astype(np.float32))]
+    for b in biases:
+        for kept in sorted({1, 2, groups // 2, groups - 1}):
+            for best in (1, 2):
+                for score in (moe_ref.SIGMOID, moe_ref.SOFTMAX):
+                    check(gpu, rows, tokens, min(8, experts), score=score, bias=b, groups=groups, groups_kept=kept, group_best=best)
