@@ -330,8 +330,8 @@ EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val,
 // the error of 32 bits, and only they are computed in 64, an expert a lane in place of all, or the groups where two of them are nearer to
 // each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly.
 //   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 15 us, 18 where two
-// groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits, where reading
-// them takes 3.3. A few tokens are one wave's chain: 64 tokens 6.1 us.
+// groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits (15.4 where a
+// softmax over all is not renormalised and each exponential is of 64 bits), where reading them takes 3.3. A few tokens are one wave's chain: 64 tokens 6.1 us.
 template <int MODE, int LPT, int VPL>
 EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, char *lds)
 {
@@ -416,10 +416,10 @@ EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane,
             }
         } else {
             if (over_all) {
-                float z = 0.0f;
+                zd = 0.0;
 #pragma unroll
-                for (int i = 0; i < VPL; ++i) z += expf(l[i] - (float)md);
-                zd = lanes_sum<LPT>(z);
+                for (int i = 0; i < VPL; ++i) zd += l[i] > -INFINITY ? exp64((double)l[i] - md) : 0.0;
+                zd = lanes_sum<LPT>(zd);
             }
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {

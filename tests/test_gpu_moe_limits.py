@@ -1,5 +1,5 @@
 """Routing to experts on the GPU (include/eif_hip_moe.h) at the ends of what scores and biases hold, against the definition in 64
-bits: sums of biases that 32 bits do not hold."""
+bits: sums of biases that 32 bits do not hold, and sums over all experts."""
 import numpy as np
 import pytest
 
@@ -62,3 +62,22 @@ def test_groups_of_lowest_biases(gpu, tokens, experts, groups):
             for best in (1, 2):
                 for score in (moe_ref.SIGMOID, moe_ref.SOFTMAX):
                     check(gpu, rows, tokens, min(8, experts), score=score, bias=b, groups=groups, groups_kept=kept, group_best=best)
+
+
+@pytest.mark.parametrize("tokens,experts,groups", [(9, 7, 1), (70, 64, 1), (2051, 64, 8), (9, 200, 1), (2051, 96, 1), (4101, 256, 8), (9, 300, 1),
+                                                   (4101, 512, 1), (9, 1000, 8), (9, 1025, 5)])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_weights_of_all_experts(gpu, tokens, experts, groups, type):
+    """A softmax over all experts is summed in 64 bits, by whichever form, and a weight rounded once."""
+    rng = np.random.default_rng(experts)
+    rows = rng.standard_normal((13, experts)).astype(np.float32)
+    rows[:4] = 1.0 + rows[:4] / 256            # near each other: each a small share of the sum
+    rows[4:7] = 40.0 + 0.25 * rows[4:7]
+    rows[7] *= 30.0
+    rows[8, rng.random(experts) < 0.5] = -np.inf
+    rows[9] = -np.inf
+    rows[10, rng.integers(experts)] = np.inf
+    rows[11] *= np.float32(1e37)
+    for scale in (1.0, 2.5):
+        check(gpu, rows, tokens, min(7, experts), type, score=moe_ref.SOFTMAX, groups=groups, groups_kept=max(1, groups // 2), renormalise=False,
+              scale=scale)
