@@ -124,7 +124,7 @@ EIF_DEV double exp64(double x)
     return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
-// 1 / d for 1 <= d < 2^1023: the instruction's 2^-26 or so and two Newton steps, each fused, so that the last rounds what it should.
+// 1 / d for 1 <= d < 2^1015: the instruction's 2^-26 or so and two Newton steps, each fused, so that the last rounds what it should.
 EIF_DEV double reciprocal(double d)
 {
     double q = __builtin_amdgcn_rcp(d);
@@ -132,11 +132,13 @@ EIF_DEV double reciprocal(double d)
     return fma(fma(-d, q, 1.0), q, q);
 }
 
-// 1 / (1 + e^-l): 0 from where e^-l leaves the range of 64 bits.
+// 1 / (1 + e^-l): 0 from where e^-l leaves the range of 64 bits (l < -1024 ln 2), and e^l below -700, where the two are the same to
+// 64 bits and the reciprocal comes near numbers that are not normal.
 EIF_DEV double sigmoid64(double l)
 {
-    const double s = reciprocal(1.0 + exp64(-larger(l, -709.7)));
-    return l < -709.7 ? 0.0 : s;
+    const bool far = l < -700.0;
+    const double e = exp64(far ? l : -l), s = far ? e : reciprocal(1.0 + e);
+    return l < -709.782712893384 ? 0.0 : s;
 }
 
 template <typename T>
@@ -331,7 +333,8 @@ EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val,
 // each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly.
 //   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 15 us, 18 where two
 // groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits (15.4 where a
-// softmax over all is not renormalised and each exponential is of 64 bits), where reading them takes 3.3. A few tokens are one wave's chain: 64 tokens 6.1 us.
+// softmax over all is not renormalised and each exponential is of 64 bits), where reading them takes 3.3. A few tokens are one wave's
+// chain: 64 tokens 6.1 us.
 template <int MODE, int LPT, int VPL>
 EIF_DEV void route_token(const RouteArgs &a, int64_t token, bool live, int lane, char *lds)
 {

@@ -43,8 +43,9 @@ size_t eif_hip_moe_sort_bytes(int tokens, int top_k, int experts);
 /* logits [tokens, ldl >= experts] of `type` (EIF_HIP_F32, _F16, _BF16; eif_hip_mx.h) -> ids [tokens, top_k] and weights
  * [tokens, top_k], a token's experts in the order of their choice.
  *   A logit of -inf or NaN, or a bias of -inf or NaN, shuts its expert out of the choice; +inf counts as the largest FP32 number.
- *   Score s: softmax over the token's logits (those of -inf and NaN count 0), or 1 / (1 + e^-l). Value v = s + bias. s and v are in
- *   64 bits. Without a bias experts are compared by their logits, in whose order the scores are; else by v.
+ *   Score s: softmax over the token's logits (those of -inf and NaN count 0), or 1 / (1 + e^-l) (0 where e^-l is more than 64 bits
+ *   hold, l below -709.78). Value v = s + bias. s and v are in 64 bits. Without a bias experts are compared by their logits, in whose
+ *   order the scores are; else by v.
  *   Groups: a group is worth the largest of what its experts are compared by, or (group_best 2) the sum of the two largest v of its
  *   experts that may be chosen (of one, that one's); the groups_kept worth most keep their experts in the choice.
  *   The top_k best of the experts left are chosen. Equals go to the lowest index, of groups and of experts.

@@ -1,5 +1,5 @@
 """Routing to experts on the GPU (include/eif_hip_moe.h) at the ends of what scores and biases hold, against the definition in 64
-bits: sums of biases that 32 bits do not hold, and sums over all experts."""
+bits: sums of biases that 32 bits do not hold, sums over all experts, and scores next to the least numbers."""
 import numpy as np
 import pytest
 
@@ -81,3 +81,21 @@ def test_weights_of_all_experts(gpu, tokens, experts, groups, type):
     for scale in (1.0, 2.5):
         check(gpu, rows, tokens, min(7, experts), type, score=moe_ref.SOFTMAX, groups=groups, groups_kept=max(1, groups // 2), renormalise=False,
               scale=scale)
+
+
+@pytest.mark.parametrize("tokens,experts,groups", [(6, 16, 4), (6, 64, 1), (6, 256, 8), (2100, 256, 8), (2100, 128, 1), (6, 1000, 10), (3, 1100, 11)])
+def test_least_scores(gpu, tokens, experts, groups):
+    """Scores next to the least numbers of 64 bits, and of them: 1 / (1 + e^-l) down to where e^-l leaves 64 bits."""
+    rng = np.random.default_rng(experts)
+    rows = np.empty((6, experts), np.float32)
+    rows[0] = rng.uniform(-712.0, -690.0, experts)
+    rows[1] = rng.uniform(-709.79, -709.69, experts)
+    rows[2] = rng.uniform(-709.0, -708.0, experts)
+    rows[3] = rng.uniform(-746.0, -709.6, experts)
+    rows[4] = -709.75
+    rows[5] = np.where(np.arange(experts) % 3 == 1, -700.0, np.where(np.arange(experts) % 3, -709.8, -699.9))
+    for b in (None, np.zeros(experts, np.float32), np.where(np.arange(experts) % 2, 0.0, -np.inf).astype(np.float32)):
+        for best in (1, 2):
+            for renormalise in (True, False):
+                check(gpu, rows, tokens, min(8, experts), score=moe_ref.SIGMOID, bias=b, groups=groups, groups_kept=max(1, groups // 2),
+                      group_best=best, renormalise=renormalise)
