@@ -1,10 +1,10 @@
 """Routing to experts on the GPU (include/eif_hip_moe.h) at the ends of what scores and biases hold, against the definition in 64
-bits: sums of biases that 32 bits do not hold, sums over all experts, and scores next to the least numbers."""
+bits: sums of biases that 32 bits do not hold, sums over all experts, scores next to the least numbers; and in the forms of many tokens."""
 import numpy as np
 import pytest
 
 import moe_ref
-from test_gpu_moe import dev, host, ints
+from test_gpu_moe import dev, host, ints, logits_of
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,28 @@ def test_least_scores(gpu, tokens, experts, groups):
             for renormalise in (True, False):
                 check(gpu, rows, tokens, min(8, experts), score=moe_ref.SIGMOID, bias=b, groups=groups, groups_kept=max(1, groups // 2),
                       group_best=best, renormalise=renormalise)
+
+
+@pytest.mark.parametrize("tokens,experts,top,groups,kept", [
+    (4999, 256, 8, 8, 4), (4999, 256, 16, 1, 1), (2300, 256, 14, 16, 9), (5001, 100, 5, 5, 3), (4097, 130, 9, 13, 6), (4113, 24, 4, 8, 3),
+    (4097, 60, 6, 60, 20), (4500, 300, 8, 10, 4), (4200, 1000, 12, 20, 7), (4103, 512, 64, 1, 1), (5003, 1024, 17, 64, 30), (4099, 1030, 6, 10, 5),
+])
+def test_long_prompts(gpu, tokens, experts, top, groups, kept):
+    """Many tokens, of workgroups with four waves, the last of them partly filled: biases that shut experts out, padding, infinities,
+    equals and near groups, of every type."""
+    rng = np.random.default_rng(tokens)
+    n = 61
+    bias = (0.2 * rng.standard_normal(experts)).astype(np.float32)
+    shut = bias.copy()
+    shut[rng.random(experts) < 0.2] = -np.inf
+    shut[rng.random(experts) < 0.1] = np.nan
+    shut[rng.integers(experts)] = np.inf
+    for i, (score, b) in enumerate(((s, b) for s in (moe_ref.SOFTMAX, moe_ref.SIGMOID) for b in (None, bias, shut))):
+        for j, (kind, type) in enumerate((("plain", "bf16"), ("ties", "f16"), ("edges", "f32"))):
+            rows = logits_of(rng, n, experts, kind)
+            check(gpu, rows, tokens, top, type, sorted_too=(i + j) % 2 == 0, score=score, bias=b, groups=groups, groups_kept=kept,
+                  group_best=1 + (i + j + i // 3) % 2 if groups < experts else 1, renormalise=(i + j) % 3 != 0, scale=(1.0, 2.5)[j % 2])
+    near = np.concatenate([20.0 + np.arange(experts)[None] * 2.0 ** -10 * s for s in (1.0, -1.0)] + [logits_of(rng, 3, experts, "plain")])
+    large = (rng.integers(-3, 4, experts) * 2.0 ** 20).astype(np.float32)
+    for b in (None, np.zeros(experts, np.float32), np.full(experts, 100.0, np.float32), large):
+        check(gpu, near.astype(np.float32), tokens, top, score=moe_ref.SIGMOID, bias=b, groups=groups, groups_kept=kept, group_best=2)
