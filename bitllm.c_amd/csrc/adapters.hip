@@ -238,8 +238,8 @@ __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
     if (n < a.rows) *y = base + out;
 }
 
-// A float as the sum of three bf16, exactly (8 bits of its 24 each), four at a time; an infinity or NaN is in the first alone. The others
-// may be 0, which an infinite factor makes NaN.
+// A float as the sum of three bf16, exactly (8 bits of its 24 each) down to bf16's least number, 2^-133, four at a time; an infinity or
+// NaN is in the first alone. The others may be 0, which an infinite factor makes NaN.
 EIF_DEV void planes4(v4f v, uint2 *p)
 {
     uint32_t h[3][4];

@@ -47,8 +47,9 @@ int eif_hip_adapters_info(const eif_hip_adapters *a, int *slots, int *rows, int 
  * worked on by itself; of more rows those that share an adapter should lie together.
  * Products and sums in FP32, in an order that M and the shapes set, not the slots of other rows. An infinity or NaN in an adapter's
  * matrices reaches outputs of the rows that name it alone, which are infinite or NaN: which of the two goes by the form, since many rows
- * are multiplied in parts, whose zeros make NaN of an infinity. One launch; nothing is allocated and nothing kept, so that any number of
- * calls may run at once and be captured into graphs. M up to 2^24, else EIF_HIP_E_LIMIT. */
+ * are multiplied in parts, whose zeros make NaN of an infinity. What of x and of A x lies below 2^-133 may be left out.
+ * One launch; nothing is allocated and nothing kept, so that any number of calls may run at once and be captured into graphs. M up to
+ * 2^24, else EIF_HIP_E_LIMIT. */
 int eif_hip_adapters_linear(const eif_hip_adapters *a, const void *x, int type, int64_t ldx, const int32_t *slot, const float *base,
                             int64_t ldbase, float *y, int64_t ldy, int M, void *stream);
 

@@ -1,4 +1,4 @@
-"""Low-rank adapters on the GPU (include/eif_hip_adapters.h) whose matrices hold infinities, in each form."""
+"""Low-rank adapters on the GPU (include/eif_hip_adapters.h) whose matrices hold infinities, and rows of the least values, in each form."""
 import numpy as np
 import pytest
 
@@ -46,3 +46,21 @@ def test_infinite_elements(gpu, types, rank, m):
     assert not np.isfinite(got[reached]).any()
     want, tol = moe_ref.adapters(x, slot, c.pairs, base, rows)
     assert (np.abs(got - want)[~reached] <= tol[~reached]).all()
+
+
+@pytest.mark.parametrize("m", [9, 600, 4100])
+@pytest.mark.parametrize("types", [("f32", "bf16"), ("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")])
+def test_least_values(gpu, types, m):
+    """Values down to the least of FP32 come through matrices of ones on the diagonal: x and A x are off by 2^-133 each at most, which is
+    what bf16 parts leave out."""
+    import torch
+    rng = np.random.default_rng(m)
+    dt = getattr(torch, TYPES[types[1]])
+    h = gpu.Adapters(1, 48, 40, 16, dt)
+    h.set(0, torch.eye(16, 40).to(dt).cuda(), torch.eye(48, 16).to(dt).cuda(), 1.0)
+    x = (rng.standard_normal((m, 40)) * 2.0 ** rng.integers(-149, -100, (m, 1))).astype(np.float32)
+    y, xd = torch.full((m, 48), 7.0, device="cuda"), dev(x, types[0])
+    h.linear(xd, dev(np.zeros(m, np.int32)), y)
+    torch.cuda.synchronize()
+    got, x = host(y).astype(np.float64), host(xd).astype(np.float64)
+    assert (np.abs(got[:, :16] - x[:, :16]) <= 2 * 2.0 ** -133 + 2.0 ** -22 * np.abs(x[:, :16])).all() and not got[:, 16:].any()
