@@ -452,6 +452,11 @@ def _ints(t, name, n):
         raise HipError(f"{name}: not {n} adjacent int32 on the device")
 
 
+def _ld(t):
+    """Elements from a row to the next one; a single row's stride means nothing, and may be less than a row."""
+    return t.stride(0) if t.shape[0] != 1 else max(t.stride(0), t.shape[1])
+
+
 def _sorted_outputs(offsets, row, slot, work, pairs, tokens, top_k, experts):
     for t, name, n in ((offsets, "offsets", experts + 1), (row, "row", pairs), (slot, "slot", pairs)):
         _ints(t, name, n)
@@ -483,7 +488,7 @@ def moe_route(logits, ids, weights, score=SCORE_SOFTMAX, bias=None, groups=1, gr
         places = _sorted_outputs(offsets, row, slot, work, tokens * top_k, tokens, top_k, experts)
     spec = MoeRouteSpec(experts=experts, top_k=top_k, score=score, bias=None if bias is None else bias.data_ptr(), groups=groups,
                         groups_kept=groups_kept, group_best=group_best, renormalise=int(renormalise), scale=scale)
-    check(load().eif_hip_moe_route(ptr(logits), _row_type(logits), logits.stride(0), tokens, C.byref(spec), ptr(ids), ptr(weights),
+    check(load().eif_hip_moe_route(ptr(logits), _row_type(logits), _ld(logits), tokens, C.byref(spec), ptr(ids), ptr(weights),
                                    *places, stream_ptr(stream)), "eif_hip_moe_route")
 
 
@@ -514,8 +519,8 @@ def moe_combine(y, slot, out, weights=None, add=None, stream=None):
             raise HipError("weights: rows of top_k adjacent elements")
     if add is not None:
         _device_tensor(add, "add", (torch.float32,), tokens, dim)
-    check(load().eif_hip_moe_combine(ptr(y), y.stride(0), y.shape[0], ptr(slot), ptr(weights), tokens, top_k, ptr(add),
-                                     0 if add is None else add.stride(0), dim, ptr(out), _row_type(out), out.stride(0),
+    check(load().eif_hip_moe_combine(ptr(y), _ld(y), y.shape[0], ptr(slot), ptr(weights), tokens, top_k, ptr(add),
+                                     0 if add is None else _ld(add), dim, ptr(out), _row_type(out), _ld(out),
                                      stream_ptr(stream)), "eif_hip_moe_combine")
 
 
@@ -569,8 +574,8 @@ class Adapters:
         _device_tensor(y, "y", (torch.float32,), m, self.rows)
         if base is not None:
             _device_tensor(base, "base", (torch.float32,), m, self.rows)
-        check(load().eif_hip_adapters_linear(self.h, ptr(x), _row_type(x), x.stride(0), ptr(slot), ptr(base),
-                                             0 if base is None else base.stride(0), ptr(y), y.stride(0), m, stream_ptr(stream)),
+        check(load().eif_hip_adapters_linear(self.h, ptr(x), _row_type(x), _ld(x), ptr(slot), ptr(base),
+                                             0 if base is None else _ld(base), ptr(y), _ld(y), m, stream_ptr(stream)),
               "eif_hip_adapters_linear")
 
 
