@@ -104,10 +104,12 @@ EIF_DEV void by_tiles(int n, F f)
 
 // A few rows: a workgroup of 16 waves has one row and 1024 of its outputs. It computes the row's whole A x, which workgroups of the
 // same row repeat (out of the XCD's L2, where they all run), and from it its outputs: one launch instead of two with the sums of the
-// first in memory between them. What a CU reads through its L1 bounds it (64 bytes a clock), so that x, which 16 lanes share, comes
-// from LDS. ONE: ranks up to 16, whose matrices are read before the rank is known (what lies behind it is zeros).
-// One row of 16 ranks through 2560x2560 3.8 us, of which 1.7 are an empty launch's and the rest a chain of slot, A and sums; 48 rows of 48
-// requests with 8 to 64 ranks through 4096x4096 11.5 us (each of a row's four workgroups reads its A, up to 512 KB).
+// first in memory between them. x, which 16 lanes share, comes from LDS, so as not to pass the L1 16 times over. ONE: ranks up to 16, whose
+// matrices are read before the rank is known (what lies behind it is zeros).
+// Bound by one workgroup's chain (slot, rank, x, A, the waves' sums, B), which grows with the ranks. One row of 16 ranks through
+// 2560x2560 3.8 us, of which 1.7 are an empty launch's. 48 rows through 4096x4096: 5.7 us with 16 ranks, 9.2 with 32, 13.4 with 64;
+// of the last, 10.5 remain with 8 rows in place of 48, 10.7 with 64 columns in place of 4096, 11.9 with 16 outputs. 48 rows of 48
+// requests with 8 to 64 ranks 11.4.
 template <typename X, typename W, bool VEC, bool ONE>
 __global__ __launch_bounds__(1024) void adapter_rows_kernel(AdapterArgs a)
 {
@@ -276,9 +278,10 @@ EIF_DEV v4f product32(const Pack<W, 8> &w, const Pack<X, 8> &x, v4f acc)
 // sums meet in LDS, where each row keeps those of its own adapter. Then base + B V, two tiles of 16 outputs at a time, with every adapter in
 // turn, each row taking its own one's. The tokens are the columns of both products. bf16 B: V as three bf16 planes on 16x16x32
 // instructions, whose products are exact, a sixteenth of the time of FP32 ones; else FP32 instructions. Loads run ahead: x and A two or
-// four steps, base and B two or three. 8192 bf16 rows of 64 ranks through 4096x4096 88 us where they share an adapter (3.8 TB/s: 25 us the
-// first product with its launch, 66 the second, copying base to y 58), 114 where nine requests meet in tiles, whose workgroups go
-// through x and the outputs for two adapters and end last. 1531 FP32 rows of 16 ranks through 6912x2560 32 us (3.1 TB/s).
+// four steps, base and B two or three. 8192 bf16 rows of 64 ranks through 4096x4096 87 us where they share an adapter (3.9 TB/s: 25 us the
+// first product with its launch, 66 the second, copying base to y 58), 113 where nine requests meet in tiles, whose workgroups go
+// through x and the outputs for two adapters and end last; 116 with f16 matrices. 1531 FP32 rows of 16 ranks through 6912x2560 31 us (3.2
+// TB/s), 28 where they share an adapter.
 template <typename X, typename W, bool VEC, int TT>
 __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(AdapterArgs a)
 {
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
                 for (int u = 0; u < DX; ++u) {
                     if (cb + u < c1) {
                         if constexpr (planes && sizeof(X) == 4) {
-                            // x as planes too: 256 rows of 64 ranks 33 us, with FP32 instructions 51; of 16 ranks as long either way
+                            // x as planes too: 1024 rows of 64 ranks 34 us, with FP32 instructions 50; of 16 ranks as long either way
 #pragma unroll
                             for (int t = 0; t < TT; ++t) {
                                 uint2 lo[3], hi[3];
@@ -450,8 +453,8 @@ __global__ __launch_bounds__(512, TT == 1 ? 4 : 2) void adapter_tile_kernel(Adap
         if (!live[t] || (s[t] < 0 && in_place)) return;
         float *y = a.y + row[t] * a.ldy;
         if (a.vec_y) {
-            // past the caches with tiles of 16 rows (1531 rows through 6912x2560 36.3 us, 39.0 without), not with those of 32 (8192 rows
-            // through 4096x4096 72 us for the second product, 68 without)
+            // past the caches with tiles of 16 rows (1531 rows through 6912x2560 31 us, 42 without), not with those of 32 (8192 rows
+            // through 4096x4096 92 us, 87 without)
             if (n < a.rows) {
                 if constexpr (TT == 1) __builtin_nontemporal_store(v, reinterpret_cast<v4f *>(y + n));
                 else *reinterpret_cast<v4f *>(y + n) = v;
@@ -609,15 +612,16 @@ int launch_tiles_as(AdapterArgs a, int workgroups, hipStream_t st)
 {
     const int tiles = eif_ceil_div(a.M, 16 * TT);
     a.tiles_xcd = eif_ceil_div(tiles, 8);
-    // workgroups that run at once: one more would begin when the others end (600 rows through 2560x2560 26.8 us with 520, 19.9 with 480)
+    // workgroups that run at once: one more would begin when the others end (600 rows through 2560x2560 25 us with 600, 19 with 480)
     a.splits = std::max(1, std::min(eif_ceil_div(a.rows, 128), workgroups / (a.tiles_xcd * 8)));
     adapter_tile_kernel<X, W, VEC, TT><<<(unsigned)(a.tiles_xcd * 8 * a.splits), 512, 0, st>>>(a);
     EIF_HIP_LAUNCHED();
     return EIF_HIP_OK;
 }
 
-// Tiles of 32 rows read A and B half as often, and leave half as many workgroups: 4096 rows of 16 ranks through 4096x4096 55 us with them,
-// 59 with tiles of 16, 8192 of 64 88 and 105; 3000 77 either way; 1531 rows of five requests through 6912x2560 51 and 48.
+// Tiles of 32 rows read A and B half as often, and leave half as many workgroups, whose stores stay in the caches. us with tiles of 32 / 16:
+// 8192 rows of 64 ranks through 4096x4096 87 / 109, with nine requests 113 / 129; 4096 of 64 57 / 67, of 16 50 / 56; 3000 bf16 rows of 64
+// ranks 52 / 41, of 16 45 / 32, FP32 rows of 16 51 / 57; 1531 rows of five requests through 6912x2560 42 / 31, 4096 of them 75 / 83.
 template <typename X, typename W, bool VEC>
 int launch_tiles(const AdapterArgs &a, hipStream_t st)
 {
@@ -629,8 +633,8 @@ int launch_adapters_as(AdapterArgs a, hipStream_t st)
 {
     const bool vec = aligned(a.x, 16) && a.ldx % 8 == 0 && a.cols % 8 == 0;
     // A row a workgroup does not care which adapters meet, a tile does (us, rows of one adapter / of 32 in any order; 512 rows of 16 ranks
-    // through 2560x2560: rows 21 / 22, tiles 18 / 88; 256 of 64 through 4096x4096 42 / 49, 33 / 397; 512 81 / 94, 35 / 427; 64 12 / 16, 29 /
-    // 296): up to the sizes of a batch of single tokens the rows.
+    // through 2560x2560: rows 20 / 21, tiles 18 / 79; 256 of 64 through 4096x4096 38 / 49, 30 / 350; 512 72 / 90, 31 / 361; 64 12 / 15, 18 /
+    // 200): up to the sizes of a batch of single tokens the rows.
     if (a.M * std::min(a.rank_tiles, 2) <= 512) {
         a.splits = eif_ceil_div(a.rows, 1024);
         const unsigned blocks = (unsigned)(eif_ceil_div(a.M, 8) * 8 * a.splits);

@@ -330,9 +330,10 @@ EIF_DEV void choose_plainly(const RouteArgs &a, int64_t row, int lane, KEY *val,
 //   The choice: the top-th largest of the lanes' largest is at most the top-th largest of all, so that the experts at or above it hold the
 // chosen ones, and are few more. They go to LDS, and each counts those that come before it. Sifted: the candidates are those within
 // the error of 32 bits, and only they are computed in 64, an expert a lane in place of all, or the groups where two of them are nearer to
-// each other than that error. Candidates beyond the room in LDS (many equals) are chosen plainly.
+// each other than that error. Candidates beyond the room in LDS are chosen plainly: many equals; of 256 experts, a third of the waves
+// where 16 lanes choose 15, and nine in ten where they choose 16 (some 48 candidates a token); most tokens where 64 lanes choose more than 44.
 //   Bound by the vector instructions, 1300 a wave of four tokens and 256 experts with a bias and groups: 16001 tokens 15 us, 18 where two
-// groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 11.7 without groups, 9.8 by logits (15.4 where a
+// groups of some token have to be told apart in 64 bits (22 with all experts in 64 bits), 12.6 without groups, 9.8 by logits (15.4 where a
 // softmax over all is not renormalised and each exponential is of 64 bits), where reading them takes 3.3. A few tokens are one wave's
 // chain: 64 tokens 6.1 us.
 template <int MODE, int LPT, int VPL>
@@ -884,7 +885,9 @@ int launch_route_as(const RouteArgs &a, const SortedTo &to, hipStream_t st)
 
 // Lanes of a token: 16, so that its fixed work is shared by four tokens of a wave, or 64 where there are few tokens, whose time is one
 // wave's (us, 16 / 64: 64 tokens of 256 experts with a bias and groups 8.9 / 6.5, without 6.9 / 4.8; 2000 9.0 / 7.2, 4000 9.3 / 9.7;
-// one token of 32 3.0 / 3.5).
+// one token of 32 3.0 / 3.5). Those are of 8 experts a token. Of 16 the candidates pass the room of 16 lanes: 16001 tokens of 256 experts by
+// logits 10.8 us for 8, 17.6 for 13, 27.6 for 16, and 14.9 for 17 on 64 lanes; sifted 12.6, 24, 40 and 17.5. 64 of 512 experts take 203 and
+// 281 us, chosen plainly.
 template <int MODE>
 int launch_route(const RouteArgs &a, const SortedTo &to, hipStream_t st)
 {

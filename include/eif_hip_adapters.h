@@ -31,8 +31,9 @@ void eif_hip_adapters_destroy(eif_hip_adapters *a);
 
 /* Puts an adapter into a slot, in the place of what it held: A [rank, lda >= cols], B [rows, ldb >= rank] of the adapters' type, host
  * pointers (src_on_device = 0; the elements between the rows are read too) or device pointers (1). rank 0 empties the slot (A and B are
- * not read). Not inside a graph capture. In the stream's order, and synchronous: it returns after the copy. Calls of
- * eif_hip_adapters_linear that are under way on other streams meanwhile must not name this slot; other slots are not touched. */
+ * not read). Not inside a graph capture. In the stream's order, and synchronous: it returns after the copy. From host memory it allocates
+ * and frees device memory for the copy, which may wait for other streams' work. Calls of eif_hip_adapters_linear that are under way on
+ * other streams meanwhile must not name this slot; other slots are not touched. */
 int eif_hip_adapters_set(eif_hip_adapters *a, int slot, int rank, const void *A, int64_t lda, const void *B, int64_t ldb, float scale,
                          int src_on_device, void *stream);
 
